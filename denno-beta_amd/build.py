@@ -43,6 +43,7 @@ LIBRARIES = {
     "attention": ("hip", ["kernels/attention.hip"], ["kernels/common.h", "kernels/attention.h"]),
     "sampling": ("hip", ["kernels/sampling.hip"], ["kernels/common.h"]),
     "sequence": ("hip", ["kernels/sequence.hip", "kernels/scan_chunks.hip"], ["kernels/common.h"]),
+    "cache8": ("hip", ["kernels/cache8.hip"], ["kernels/common.h", "kernels/cache8.h"]),
     "grouped": ("hip", ["kernels/grouped.hip"], ["kernels/common.h"]),
 }
 

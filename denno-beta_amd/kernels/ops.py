@@ -177,6 +177,10 @@ def _declare(name, lib):
             "dn_moe_down": [P, I, P, P, I, I, P, I, I, I, P, I, P],
             "dn_moe_combine": [P, P, c_longlong, I, I, I, I, P, c_longlong, P, I, P, I, c_longlong, P],
         },
+        "cache8": {
+            "dn_kv_append8": [P, I, I, I, P, P, P, P, P, I, P, P, I, I, F, I, I, P, I, I, I, I, I, I, P],
+            "dn_attention8": [P, I, P, I, P, P, P, P, I, P, I, P, P, P, P, I, I, I, I, I, F, I, I, I, P, F, I, P],
+        },
         "sampling": {
             "dn_sample": [P, I, I, I, P, P, P, P],
             "dn_penalties": [P, I, I, I, P, P, P, P, P, P, P, P],
@@ -865,6 +869,120 @@ def attention(q, out, k_pool, v_pool, block_tables, tiles, n_heads, scale, windo
         block_tables.shape[1], base, base + 4 * n_tiles, base + 8 * n_tiles, base + 12 * n_tiles, n_tiles,
         n_heads, Hkv, dh, ps, float(scale), int(window), int(chunk), _ptr(bias), span, int(sink), _ptr(sink_at), keep_first,
         float(softcap), _CODE[q.dtype], _stream()), "attention")
+    return out
+
+
+def _pools8(k_pool, v_pool, k_scale, v_scale, what):
+    """The cache in 8 bits: -> (n_pages, Hkv, page_size, dh)."""
+    _dev(k_pool, "k_pool", (torch.float8_e4m3fn,), 4), _dev(v_pool, "v_pool", (torch.float8_e4m3fn,), 4)
+    _dev(k_scale, "k_scale", (torch.float32,), 2), _dev(v_scale, "v_scale", (torch.float32,), 2)
+    n_pages, Hkv, ps, dh = k_pool.shape
+    _need(k_pool.is_contiguous() and v_pool.is_contiguous() and tuple(v_pool.shape) == (n_pages, Hkv, dh, ps),
+          lambda: f"{what}: pools {tuple(k_pool.shape)} and {tuple(v_pool.shape)}; wanted [pages, heads, page, dim] and [pages, heads, dim, page]")
+    for t in (k_scale, v_scale):
+        _need(t.is_contiguous() and tuple(t.shape) == (n_pages, Hkv), lambda: f"{what}: a scale per page and head, not {tuple(t.shape)}")
+    _need(n_pages >= 1 and Hkv >= 1 and ps >= 1, lambda: f"{what}: empty pools")
+    _need(1 <= dh <= 256, lambda: f"{what}: head size {dh} must be at most 256")
+    return n_pages, Hkv, ps, dh
+
+
+def _one_device(what, first, *others):
+    """All on one device, and that the current one: a launch goes to the current device's stream."""
+    for t in others:
+        _need(t is None or t.device == first.device, lambda: f"{what}: tensors on {first.device} and {t.device}")
+    _need(first.device.index == torch.cuda.current_device(), lambda: f"{what}: tensors on {first.device}, which is not the current device")
+
+
+def kv_append8(src, k_col, v_col, slot_map, k_pool, v_pool, k_scale, v_scale, positions=None, freq=None, halves=False, mag=1.0,
+               q_out=None, q_col=0, n_heads=0):
+    """A step's keys and values to the pages of a cache in 8 bits, keys (and queries) turned by their positions on the way.
+
+    src: [T, ld], 32-bit or bfloat16; a row's keys stand at columns k_col.., its values at v_col..; slot_map[t] = page * page_size + place
+    (negative: the row's keys and values go nowhere).  The rows of one page stand side by side, as a step's do, and no slot comes twice.
+    k_pool: e4m3 [n_pages, Hkv, page_size, dh]; v_pool: e4m3 [n_pages, Hkv, dh, page_size]; k_scale, v_scale: 32-bit [n_pages, Hkv]: a
+    number of a page and head stands for itself times that scale, a power of two.
+
+    In a page and head that gets rows: a row in the page's first place begins it anew (nothing it held counts, its other places become
+    zero); the scale 2^e is the least with which the largest new magnitude is at most 448, e at least -117, and no less than the scale
+    that the page has, unless it begins anew; new numbers are the nearest to value / 2^e, ties to the even one; where the scale grew
+    what the page held is rounded in the same way.  A value that is not finite is kept as NaN and does not count for the scale.
+
+    freq: 32-bit [dims / 2]: the first `dims` entries of every key are turned in pairs, entries 2i and 2i + 1, or with halves i and
+    i + dims / 2, by the angle positions[t] * freq[i] (cos and sin times mag; in 64 bits until the one rounding).  q_out [T, n_heads * dh] of src's
+    dtype: the queries at columns q_col.. of src, turned the same way (it may be those columns themselves)."""
+    _dev(src, "src", _FLOATS, 2), _dev(slot_map, "slot_map", _I32, 1)
+    n_pages, Hkv, ps, dh = _pools8(k_pool, v_pool, k_scale, v_scale, "kv_append8")
+    ld, T, w = _rows(src, "src"), src.shape[0], Hkv * dh
+    _need(slot_map.is_contiguous() and slot_map.shape[0] == T, "kv_append8: slot_map")
+    _need(0 <= k_col and k_col + w <= src.shape[1] and 0 <= v_col and v_col + w <= src.shape[1], "kv_append8: columns outside src")
+    _one_device("kv_append8", src, slot_map, k_pool, v_pool, k_scale, v_scale, positions, freq, q_out)
+    dims = 0
+    if freq is not None:
+        _f32vec(freq, "freq")
+        dims = 2 * freq.numel()
+        _need(2 <= dims <= dh, lambda: f"kv_append8: {freq.numel()} frequencies for heads of {dh}")
+        _need(positions is not None, "kv_append8: a turn needs positions")
+        _dev(positions, "positions", _I32, 1)
+        _need(positions.is_contiguous() and positions.shape[0] == T, "kv_append8: positions")
+    ldq = 0
+    if q_out is not None:
+        _need(dims > 0, "kv_append8: queries are only turned here; without a turn they are src's own columns")
+        _dev(q_out, "q_out", (src.dtype,), 2)
+        qw = n_heads * dh
+        _need(n_heads >= 1 and tuple(q_out.shape) == (T, qw) and 0 <= q_col and q_col + qw <= src.shape[1], "kv_append8: queries")
+        _need(q_col + qw <= min(k_col, v_col) or q_col >= max(k_col, v_col) + w or (k_col + w <= q_col and q_col + qw <= v_col)
+              or (v_col + w <= q_col and q_col + qw <= k_col), "kv_append8: the queries' columns are keys' or values' too")
+        ldq = _rows(q_out, "q_out")
+        size = src.element_size()
+        there, first, own_first = q_out.data_ptr() == src.data_ptr() + q_col * size and (ldq == ld or T == 1), q_out.data_ptr(), src.data_ptr()
+        _need(there or T == 0 or first >= own_first + ((T - 1) * ld + src.shape[1]) * size or first + ((T - 1) * ldq + qw) * size <= own_first,
+              "kv_append8: q_out is either src's own query columns or memory apart from src")
+    else:
+        _need(n_heads == 0, "kv_append8: n_heads goes with q_out")
+    if T == 0:
+        return
+    _ok(_lib("cache8").dn_kv_append8(src.data_ptr(), ld, k_col, v_col, slot_map.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(),
+                                     k_scale.data_ptr(), v_scale.data_ptr(), n_pages, _ptr(positions if dims else None), _ptr(freq), dims,
+                                     int(bool(halves)), float(mag), q_col, n_heads, _ptr(q_out), ldq, T, Hkv, dh, ps, _CODE[src.dtype],
+                                     _stream()), "kv_append8")
+
+
+def attention8(q, out, k_pool, v_pool, k_scale, v_scale, block_tables, tiles, n_heads, scale, window=0, tiles_wide=None,
+               single_rows=False, max_context=0, sink=False, keep_first=0, softcap=0.0):
+    """`attention` over a cache in 8 bits as `kv_append8` fills it (that function has the layout of pools and scales): causal attention of
+    the batch's rows, with the same tables.
+
+    q: [T, >= H*dh], 32-bit or bfloat16, rows contiguous, head h at columns h*dh..; out: [T, H*dh] of q's dtype; query head h reads key head
+    h // (H // Hkv).  tiles: int32 [4, n_tiles] = (request, first row, rows <= 16, first position), request < 0: padding;
+    tiles_wide: the same rows cut into tiles of up to 128 rows; single_rows: a pure decode step: request s brings row s and is
+    tile s, (s or -1, s, 1, position); max_context: the longest context then.
+    window > 0: the row at position p reads the keys from p - window + 1 on, and with keep_first the request's first so many as well;
+    sink: True: one more summand exp(0) under the softmax, or 32-bit [H]: exp(sink[h]), which nothing scales; softcap > 0: a scaled score s
+    becomes softcap * tanh(s / softcap).
+    Rows of padding tiles are left as they were.  What stands in places that a row does not read does not reach it, NaN included;
+    a page that is given back (a negative entry) is not read; a row that reads nothing becomes zeros."""
+    _dev(q, "q", _FLOATS, 2), _dev(out, "out", (q.dtype,), 2)
+    n_pages, Hkv, ps, dh = _pools8(k_pool, v_pool, k_scale, v_scale, "attention8")
+    _dev(block_tables, "block_tables", _I32, 2), _dev(tiles, "tiles", _I32, 2)
+    T = q.shape[0]
+    _need(n_heads >= 1 and n_heads % Hkv == 0, lambda: f"attention8: {n_heads} heads over {Hkv} key heads")
+    _need(q.shape[1] >= n_heads * dh and tuple(out.shape) == (T, n_heads * dh), "attention8: q/out shapes")
+    _need(block_tables.is_contiguous() and tiles.is_contiguous() and tiles.shape[0] == 4, "attention8: tables")
+    ldq, ldo = _rows(q, "q"), _rows(out, "out")
+    sink_at, sink = (sink, True) if isinstance(sink, torch.Tensor) else (None, bool(sink))
+    _f32vec(sink_at, "sink", n_heads)
+    _need(window >= 0 and softcap >= 0, "attention8: window or softcap")
+    keep_first = int(keep_first) if window > 0 else 0      # (without a window every key is read anyway)
+    _need(keep_first >= 0, "attention8: keep_first")
+    _one_device("attention8", q, out, k_pool, v_pool, k_scale, v_scale, block_tables, tiles, tiles_wide, sink_at)
+    n_tiles = tiles.shape[1]
+    if T == 0 or n_tiles == 0:
+        return out
+    base = tiles.data_ptr()
+    _ok(_lib("cache8").dn_attention8(
+        q.data_ptr(), ldq, out.data_ptr(), ldo, k_pool.data_ptr(), v_pool.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), n_pages,
+        block_tables.data_ptr(), block_tables.shape[1], base, base + 4 * n_tiles, base + 8 * n_tiles, base + 12 * n_tiles, n_tiles, n_heads,
+        Hkv, dh, ps, float(scale), int(window), keep_first, int(sink), _ptr(sink_at), float(softcap), _CODE[q.dtype], _stream()), "attention8")
     return out
 
 
