@@ -1,0 +1,61 @@
+// Shared by the matrix-core kernels of attention over the cache in 8 bits (attention8_single.hip, attention8_portions.hip).
+#pragma once
+#include "cache8.h"
+
+namespace attend8 {
+
+typedef __attribute__((__vector_size__(8 * sizeof(__bf16)))) __bf16 bf16x8;
+typedef __attribute__((__vector_size__(2 * sizeof(__bf16)))) __bf16 bf16x2;
+typedef __attribute__((__vector_size__(4 * sizeof(uint32_t)))) uint32_t u32x4;
+typedef __attribute__((__vector_size__(4 * sizeof(float)))) float floatx4;
+typedef __attribute__((__vector_size__(2 * sizeof(float)))) float floatx2;
+
+constexpr float LOG2E = 1.44269504088896340736f;
+// what a running maximum starts from: below any score, and finite, so that differences of it are numbers
+constexpr float LOWEST = -3.0e38f;
+
+// eight e4m3 numbers, as they lie in two words, in bfloat16: exact
+__device__ __forceinline__ bf16x8 widen(uint32_t lo, uint32_t hi) {
+  u32x4 w;
+  w[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.0f, false));
+  w[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.0f, true));
+  w[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.0f, false));
+  w[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.0f, true));
+  return __builtin_bit_cast(bf16x8, w);
+}
+
+// eight numbers in bfloat16, two per conversion, to nearest
+__device__ __forceinline__ bf16x8 to_bf16x8(const float* v) {
+  u32x4 w;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) w[i] = __builtin_bit_cast(uint32_t, __builtin_convertvector(floatx2{v[2 * i], v[2 * i + 1]}, bf16x2));
+  return __builtin_bit_cast(bf16x8, w);
+}
+
+// Eight 32-bit numbers as PARTS numbers of bfloat16 whose sum they are: each part is what the parts before leave, rounded.  Three
+// parts hold all 24 digits of a number, so a product of 32-bit rows with the cache (whose numbers are exact in bfloat16) is three
+// products on the matrix cores with nothing lost but the 32-bit sums' own roundings; one part is a rounding to bfloat16.
+template <int PARTS>
+__device__ __forceinline__ void split(const float* v, bf16x8* parts) {
+  float rest[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) rest[i] = v[i];
+#pragma unroll
+  for (int p = 0; p < PARTS; ++p) {
+    parts[p] = to_bf16x8(rest);
+    if (p + 1 < PARTS) {
+      const u32x4 w = __builtin_bit_cast(u32x4, parts[p]);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) rest[i] -= __uint_as_float((i & 1) ? w[i / 2] & 0xffff0000u : w[i / 2] << 16);
+    }
+  }
+}
+
+// cap * tanh(s / cap) of a score in units of log2(e): s2 = s log2(e), cap2 = cap log2(e), to_tanh = 2 / cap.  tanh(x) = 1 - 2 / (e^2x + 1),
+// whose error near 0 is some 1e-7 of 1, so the score's is some 1e-7 of cap
+__device__ __forceinline__ float capped(float s2, float cap2, float to_tanh) {
+  const float e = __builtin_amdgcn_exp2f(s2 * to_tanh);
+  return cap2 * fmaf(-2.0f, __builtin_amdgcn_rcpf(e + 1.0f), 1.0f);
+}
+
+}  // namespace attend8

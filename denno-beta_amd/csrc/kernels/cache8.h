@@ -26,4 +26,13 @@ int dn_attention8(const void* q, int ldq, void* out, int ldo, const void* k_pool
                   const int32_t* tile_row0, const int32_t* tile_nrows, const int32_t* tile_pos0, int n_tiles, int H, int Hkv, int dh,
                   int page_size, float scale, int window, int keep, int sink, const float* sink_at, float cap, int dtype,
                   hipStream_t stream);
+
+// The same on the matrix cores for steps of single rows (a tile a row): head sizes that are multiples of 16, pages of a multiple of 16
+// keys, pools and rows 16-byte aligned.  Workgroups of 4 waves, or 8 up to a head size of 128; n_splits > 1: a row's keys are shared out
+// to so many workgroups, and part holds their results, n_tiles * H * n_splits * (dh + 2) floats.
+int dn_attention8_single(const void* q, int ldq, void* out, int ldo, const void* k_pool, const void* v_pool, const float* k_scale,
+                         const float* v_scale, int n_pages, const int32_t* block_tables, int max_blocks, const int32_t* tile_seq,
+                         const int32_t* tile_row0, const int32_t* tile_pos0, int n_tiles, float* part, int n_splits, int waves, int H,
+                         int Hkv, int dh, int page_size, float scale, int window, int keep, int sink, const float* sink_at, float cap,
+                         int dtype, hipStream_t stream);
 }

@@ -179,6 +179,7 @@ def _declare(name, lib):
         },
         "cache8": {
             "dn_kv_append8": [P, I, I, I, P, P, P, P, P, I, P, P, I, I, F, I, I, P, I, I, I, I, I, I, P],
+            "dn_attention8_single": [P, I, P, I, P, P, P, P, I, P, I, P, P, P, I, P, I, I, I, I, I, I, F, I, I, I, P, F, I, P],
             "dn_attention8": [P, I, P, I, P, P, P, P, I, P, I, P, P, P, P, I, I, I, I, I, F, I, I, I, P, F, I, P],
         },
         "sampling": {
@@ -947,6 +948,16 @@ def kv_append8(src, k_col, v_col, slot_map, k_pool, v_pool, k_scale, v_scale, po
                                      _stream()), "kv_append8")
 
 
+def _single8_shape(n_tiles, n_heads, Hkv, dh, max_context, window, keep_first):
+    """-> (waves of a workgroup, workgroups that a row's keys are shared out to)."""
+    reach = max_context if window == 0 else min(max_context, window + keep_first + 128)
+    tiles = -(-reach // 64)
+    groups = n_tiles * Hkv * -(-(n_heads // Hkv) // 16)
+    waves = 8 if dh <= 128 and groups < 1024 and tiles > 4 else 4
+    n_splits = max(1, min(-(-tiles // waves), 1024 // groups))
+    return waves, n_splits
+
+
 def attention8(q, out, k_pool, v_pool, k_scale, v_scale, block_tables, tiles, n_heads, scale, window=0, tiles_wide=None,
                single_rows=False, max_context=0, sink=False, keep_first=0, softcap=0.0):
     """`attention` over a cache in 8 bits as `kv_append8` fills it (that function has the layout of pools and scales): causal attention of
@@ -979,6 +990,19 @@ def attention8(q, out, k_pool, v_pool, k_scale, v_scale, block_tables, tiles, n_
     if T == 0 or n_tiles == 0:
         return out
     base = tiles.data_ptr()
+    aligned = (dh % 16 == 0 and ps % 16 == 0 and k_pool.data_ptr() % 16 == 0 and v_pool.data_ptr() % 16 == 0)
+    if single_rows and max_context > 0:
+        _need(n_tiles == T, "attention8: a step of single rows has a tile for every row")
+        _need(max_context <= block_tables.shape[1] * ps, "attention8: max_context exceeds the block tables")
+        if aligned:
+            waves, n_splits = _single8_shape(n_tiles, n_heads, Hkv, dh, max_context, window, keep_first)
+            part = torch.empty(n_tiles * n_heads * n_splits * (dh + 2), dtype=torch.float32, device=q.device) if n_splits > 1 else None
+            _ok(_lib("cache8").dn_attention8_single(
+                q.data_ptr(), ldq, out.data_ptr(), ldo, k_pool.data_ptr(), v_pool.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
+                n_pages, block_tables.data_ptr(), block_tables.shape[1], base, base + 4 * n_tiles, base + 12 * n_tiles, n_tiles, _ptr(part),
+                n_splits, waves, n_heads, Hkv, dh, ps, float(scale), int(window), keep_first, int(sink), _ptr(sink_at), float(softcap),
+                _CODE[q.dtype], _stream()), "attention8 (single rows)")
+            return out
     _ok(_lib("cache8").dn_attention8(
         q.data_ptr(), ldq, out.data_ptr(), ldo, k_pool.data_ptr(), v_pool.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), n_pages,
         block_tables.data_ptr(), block_tables.shape[1], base, base + 4 * n_tiles, base + 8 * n_tiles, base + 12 * n_tiles, n_tiles, n_heads,
