@@ -43,7 +43,7 @@ LIBRARIES = {
     "attention": ("hip", ["kernels/attention.hip"], ["kernels/common.h", "kernels/attention.h"]),
     "sampling": ("hip", ["kernels/sampling.hip"], ["kernels/common.h"]),
     "sequence": ("hip", ["kernels/sequence.hip", "kernels/scan_chunks.hip"], ["kernels/common.h"]),
-    "cache8": ("hip", ["kernels/cache8.hip", "kernels/attention8_single.hip"],
+    "cache8": ("hip", ["kernels/cache8.hip", "kernels/attention8_single.hip", "kernels/attention8_portions.hip"],
                ["kernels/common.h", "kernels/cache8.h", "kernels/attention8_common.h"]),
     "grouped": ("hip", ["kernels/grouped.hip"], ["kernels/common.h"]),
 }

@@ -1,0 +1,409 @@
+// Attention over the cache in 8 bits for portions of prompts: two products of the rows with the keys and the values, so the matrix
+// instructions are what it takes, and what stands between them (widening the cache's numbers, the softmax) has to be little.
+//
+// A workgroup takes up to RG x 32 rows of one request and one head: wave w owns 32 of them (row group w % RG), and its KG
+// key groups (w / RG) share out the keys, 64 by 64, and join at the end.  A group's tile of 64 keys comes from the pages 16 bytes a thread,
+// is widened to bfloat16 times its page's scale on the way into LDS (v_cvt_scalef32_pk_bf16_fp8: the scale, a power of two,
+// costs nothing there and nothing behind), and serves all row groups; two tiles deep, the one after the next on its way to registers.
+//   S^T = K Q^T by v_mfma_f32_32x32x16_bf16: lane (column: a row of q; half g) gets 16 keys of every 32, so the running softmax is
+//   inside a lane but for one exchange between the halves, and its weights are, eight by eight, B operands of
+//   O^T += V^T P^T, whose k-th slots are the keys 16 a + 4 g + {0..3, 8..11}: the values lie in LDS in that order, 16 bytes a read.
+// 32-bit rows: three bfloat16 parts of the queries and of the weights (attend8::split), three products for one.
+#include "attention8_common.h"
+
+namespace portions8 {
+using namespace attend8;
+typedef __attribute__((__vector_size__(16 * sizeof(float)))) float floatx16;
+
+struct Args {
+  const void* q;
+  void* out;
+  const uint8_t *k_pool, *v_pool;
+  const float *k_scale, *v_scale;
+  const int32_t *block_tables, *tile_seq, *tile_row0, *tile_nrows, *tile_pos0;
+  const float* sink_at;
+  int ldq, ldo, n_pages, max_blocks, H, Hkv, page_size, window, keep, sink;
+  float scale, cap;
+};
+
+__device__ __forceinline__ u32x4 widen_scaled(uint32_t lo, uint32_t hi, float scale) {
+  u32x4 w;
+  w[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, scale, false));
+  w[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, scale, true));
+  w[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, scale, false));
+  w[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, scale, true));
+  return w;
+}
+
+// A wait for products that are read behind a branch, which the compiler does not always leave room for: 16 cycles, as a product of 32 x 32 wants at least
+__device__ __forceinline__ void settle(floatx16& a, floatx16& b) { asm volatile("s_nop 15" : "+v"(a), "+v"(b)); }
+
+// whether one of a word's four e4m3 numbers is NaN (0x7f or 0xff)
+__device__ __forceinline__ uint32_t nan_in(uint32_t w) { return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
+
+template <int DH16, int PARTS, int RG, int KG>
+constexpr int waves_per_simd() {      // (with room for one wave only, the compiler moves results to and fro between two sets of registers)
+  return DH16 * (4 * PARTS + 8) > 128 ? 1 : 2;
+}
+
+template <int DH16, int PARTS, int RG, int KG>
+__global__ __launch_bounds__(64 * RG * KG) __attribute__((amdgpu_waves_per_eu(waves_per_simd<DH16, PARTS, RG, KG>()))) void kernel(const Args a) {
+  constexpr int DH = DH16 * 16, DB = (DH + 31) / 32;
+  constexpr int KROW = DH + 8, VROW = 72;                // elements of a key's row, of a dim's row of 64 keys, 16 bytes of padding each
+  constexpr int KSZ = 64 * KROW, TSZ = KSZ + DH * VROW;  // of a tile's keys, of a tile
+  constexpr int THREADS = 64 * RG;                       // of a key group
+  constexpr int CHUNKS = 64 * DH16;                      // 16-byte chunks of a tile's keys, and of its values
+  constexpr int U = (CHUNKS + THREADS - 1) / THREADS;
+  constexpr int JOIN = 2 + 16 * DB;
+  constexpr int BYTES_TILES = 2 * KG * TSZ * 2, BYTES_JOIN = (KG - 1) * THREADS * JOIN * 4;
+  constexpr int SUBS = 4 / RG;
+  extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+  bf16_t* const tiles = reinterpret_cast<bf16_t*>(smem);                        // [2][KG][keys | values]
+  constexpr int FLAGS_AT = BYTES_TILES > BYTES_JOIN ? BYTES_TILES : BYTES_JOIN;
+  int* const flags = reinterpret_cast<int*>(smem + FLAGS_AT);                   // [2][KG][4 blocks: whether there is a page | RG waves: NaN among values]
+
+  // consecutive workgroups go to different XCDs: the heads of one key head are Hkv workgroups apart, so that with 8 key heads (or a
+  // multiple) an XCD's L2 holds the keys of its own heads only
+  const int G = a.H / a.Hkv;
+  const int hk = blockIdx.x % a.Hkv, h = hk * G + blockIdx.x / a.Hkv;
+  const int tile = blockIdx.y / SUBS, sub = SUBS - 1 - blockIdx.y % SUBS;      // (the longest first)
+  const int seq = a.tile_seq[tile];
+  const int r0 = sub * 32 * RG;
+  const int nrows = min(a.tile_nrows[tile] - r0, 32 * RG);
+  if (seq < 0 || nrows <= 0) return;      // the whole workgroup
+  const int row0 = a.tile_row0[tile] + r0, pos0 = a.tile_pos0[tile] + r0;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64;
+  const int kg = wave / RG, rg = wave % RG, t = threadIdx.x % THREADS;
+  const int col = lane % 32, g = lane / 32;
+  const int ps = a.page_size;
+  const int32_t* bt = a.block_tables + static_cast<size_t>(seq) * a.max_blocks;
+  const int wrow0 = rg * 32;
+  const bool has_rows = wrow0 < nrows;      // (a wave without rows carries tiles all the same)
+  const bool row_ok = wrow0 + col < nrows;
+  const int my_row = min(wrow0 + col, nrows - 1), my_pos = pos0 + my_row;
+  auto first_key = [&](int pos) { return a.window > 0 ? max(0, pos - a.window + 1) : 0; };
+  const int my_lo = first_key(my_pos), lo_w = first_key(pos0 + wrow0), hi_w = pos0 + min(wrow0 + 31, nrows - 1), lo_last = first_key(hi_w);
+  const int lo_g = first_key(pos0), hi_g = pos0 + nrows - 1, lo_g_last = first_key(hi_g);
+
+  bf16x8 qf[DH16][PARTS];
+#pragma unroll
+  for (int c = 0; c < DH16; ++c) {
+    const size_t at = static_cast<size_t>(row0 + my_row) * a.ldq + h * DH + c * 16 + g * 8;
+    if constexpr (PARTS == 1) {
+      qf[c][0] = *reinterpret_cast<const bf16x8*>(static_cast<const bf16_t*>(a.q) + at);
+    } else {
+      float v[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = static_cast<const float*>(a.q)[at + j];
+      split<PARTS>(v, qf[c]);
+    }
+  }
+  floatx16 o[DB];
+#pragma unroll
+  for (int d = 0; d < DB; ++d)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) o[d][i] = 0.f;
+  float m_run = LOWEST, l_run = 0.f;
+  const float scale2 = a.scale * LOG2E, cap2 = a.cap * LOG2E, to_tanh = a.cap > 0.f ? 2.0f / a.cap : 0.f;
+  const float per_score = a.cap > 0.f ? 1.0f : scale2;      // what is left to multiply a score with
+
+  // Steps of 64 KG keys: `kept` ones from the start, then those from the window's first key on.  Step i begins with key_of(i).
+  constexpr int STEP = 64 * KG;
+  const int kept = a.keep > 0 ? (min(a.keep, hi_g + 1) + STEP - 1) / STEP : 0;
+  const int rest = max(lo_g / STEP, kept);
+  const int steps = kept + max(0, hi_g / STEP - rest + 1);
+  auto key_of = [&](int i) { return STEP * (i < kept ? i : rest + i - kept); };
+
+  // This thread's chunks of its group's tile: chunk x = t + THREADS u is, of the keys, 16 dims (x % DH16) of key x / DH16; of the
+  // values, the 16 keys of block x % 4 of dim x / 4 (the same block for every u).
+  auto page_of = [&](int key) {      // of the block of 16 that begins with key; -1: none, or behind the last row
+    const int b = key / ps;
+    const int page = key <= hi_g && b < a.max_blocks ? bt[b] : -1;
+    return page < a.n_pages ? page : -1;
+  };
+  int k_page[U], v_page;
+  u32x4 k_raw[U], v_raw[U];
+  float k_by[U], v_by;
+  int k_key[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) k_key[u] = min(t + THREADS * u, CHUNKS - 1) / DH16;
+  auto pages = [&](int i) {
+    const int kt = key_of(i) + 64 * kg;
+#pragma unroll
+    for (int u = 0; u < U; ++u) k_page[u] = i < steps ? page_of(kt + (k_key[u] & ~15)) : -1;
+    v_page = i < steps ? page_of(kt + 16 * (t % 4)) : -1;
+  };
+  int v_there = 0;      // whether the values in registers have a page
+  auto fetch = [&](int i) {      // (what has no page reads the pools' first and is stored as zeros)
+    const int kt = key_of(i) + 64 * kg;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const size_t ph = static_cast<size_t>(max(k_page[u], 0)) * a.Hkv + hk;
+      k_raw[u] = *reinterpret_cast<const u32x4*>(a.k_pool + (ph * ps + (kt + k_key[u]) % ps) * DH + min(t + THREADS * u, CHUNKS - 1) % DH16 * 16);
+      k_by[u] = a.k_scale[ph];
+      if (k_page[u] < 0) k_by[u] = -1.f;      // (settled when the chunk is stored)
+    }
+    const size_t ph = static_cast<size_t>(max(v_page, 0)) * a.Hkv + hk;
+    v_by = a.v_scale[ph];
+    v_there = v_page >= 0;
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      v_raw[u] = *reinterpret_cast<const u32x4*>(a.v_pool + (ph * DH + min(t + THREADS * u, CHUNKS - 1) / 4) * ps + (kt + 16 * (t % 4)) % ps);
+  };
+  const u32x4 zero4 = {0u, 0u, 0u, 0u};
+  auto stash = [&](int i, int buf) {
+    bf16_t* dst = tiles + (buf * KG + kg) * TSZ;
+    int* flag = flags + (buf * KG + kg) * (4 + RG);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int x = t + THREADS * u;
+      if (CHUNKS % THREADS == 0 || x < CHUNKS) {
+        const bool ok = k_by[u] >= 0.f;
+        u32x4* to = reinterpret_cast<u32x4*>(dst + x / DH16 * KROW + x % DH16 * 16);
+        to[0] = ok ? widen_scaled(k_raw[u][0], k_raw[u][1], k_by[u]) : zero4;
+        to[1] = ok ? widen_scaled(k_raw[u][2], k_raw[u][3], k_by[u]) : zero4;
+      }
+    }
+    uint32_t nan = 0;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int x = t + THREADS * u;
+      if (CHUNKS % THREADS == 0 || x < CHUNKS) {
+        u32x4* to = reinterpret_cast<u32x4*>(dst + KSZ + x / 4 * VROW + x % 4 * 16);
+        to[0] = v_there ? widen_scaled(v_raw[u][0], v_raw[u][2], v_by) : zero4;
+        to[1] = v_there ? widen_scaled(v_raw[u][1], v_raw[u][3], v_by) : zero4;
+        nan |= nan_in(v_raw[u][0]) | nan_in(v_raw[u][1]) | nan_in(v_raw[u][2]) | nan_in(v_raw[u][3]);
+      }
+    }
+    if (t < 4) flag[t] = v_there;
+    const uint64_t any = __builtin_amdgcn_ballot_w64((nan != 0) & (v_there != 0));
+    if (lane == 0) flag[4 + rg] = any != 0;
+  };
+
+  pages(0);
+  fetch(0);
+  pages(1);
+  stash(0, 0);
+  fetch(1);
+  pages(2);
+  __syncthreads();
+  int buf = 0;
+  for (int i = 0; i < steps; ++i, buf ^= 1) {
+    if (i + 1 < steps) stash(i + 1, buf ^ 1);
+    if (i + 2 < steps) fetch(i + 2);
+    pages(i + 3);
+
+    const int kw = key_of(i) + 64 * kg;
+    // a tile that no row of the wave reads is stepped over
+    if (has_rows && kw <= hi_w && (kw + 63 >= lo_w || kw < a.keep)) {
+      const bf16_t* Kb = tiles + (buf * KG + kg) * TSZ;
+      const bf16_t* Vb = Kb + KSZ;
+      const int* flag = flags + (buf * KG + kg) * (4 + RG);
+      const floatx16 zero16 = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+      floatx16 s[2];
+#pragma unroll
+      for (int c = 0; c < 2; ++c)
+#pragma unroll
+        for (int d = 0; d < DH16; ++d) {
+          const bf16x8 kf = *reinterpret_cast<const bf16x8*>(Kb + (32 * c + col) * KROW + d * 16 + g * 8);
+#pragma unroll
+          for (int p = 0; p < PARTS; ++p) s[c] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, qf[d][p], d == 0 && p == 0 ? zero16 : s[c], 0, 0, 0);
+        }
+      // s[c][i]: key kw + 32 c + 8 (i / 4) + 4 g + i % 4 of this lane's row
+      settle(s[0], s[1]);
+      const int there = __builtin_amdgcn_readfirstlane(flag[0] | flag[1] << 1 | flag[2] << 2 | flag[3] << 3);      // blocks with a page
+      // an edge: a key that one of the wave's rows does not read.  The same for the whole wave.
+      const bool edge = kw + 63 > pos0 + wrow0 || (kw < lo_last && kw + 63 >= a.keep) || there != 15;
+      // whether this lane's row reads its i-th key of the half tile c (no branches: all of it is one comparison after the other)
+      auto reads = [&](int c, int i) {
+        const int key = kw + 32 * c + 8 * (i / 4) + 4 * g + i % 4;
+        return ((there >> (2 * c + i / 8) & 1) != 0) & (key <= my_pos) & ((key >= my_lo) | (key < a.keep));
+      };
+      if (a.cap > 0.f) {
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) s[c][i] = capped(s[c][i] * scale2, cap2, to_tanh);
+      }
+      if (edge) {
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) s[c][i] = reads(c, i) ? s[c][i] : -INFINITY;
+      }
+      float top = LOWEST;
+#pragma unroll
+      for (int c = 0; c < 2; ++c)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) top = fmaxf(top, s[c][i]);
+      top = fmaxf(top, other_half(top));
+      const float m_new = fmaxf(m_run, top * per_score), alpha = __builtin_amdgcn_exp2f(m_run - m_new);
+      m_run = m_new;
+      float sum = 0.f;
+#pragma unroll
+      for (int c = 0; c < 2; ++c)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          s[c][i] = __builtin_amdgcn_exp2f(fmaf(s[c][i], per_score, -m_new));
+          sum += s[c][i];
+        }
+      l_run = l_run * alpha + sum;
+      if (__builtin_amdgcn_ballot_w64(alpha != 1.f) != 0) {
+#pragma unroll
+        for (int d = 0; d < DB; ++d)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) o[d][i] *= alpha;
+      }
+      int nan = 0;
+#pragma unroll
+      for (int w = 0; w < RG; ++w) nan |= flag[4 + w];
+      nan = edge ? __builtin_amdgcn_readfirstlane(nan) : 0;
+#pragma unroll
+      for (int c = 0; c < 2; ++c)
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          float p[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) p[j] = s[c][8 * x + j];
+          bf16x8 pf[PARTS];
+          split<PARTS>(p, pf);
+          if (nan == 0) {
+#pragma unroll
+            for (int d = 0; d < DB; ++d) {
+              const bf16x8 vf = *reinterpret_cast<const bf16x8*>(Vb + min(32 * d + col, DH - 1) * VROW + 32 * c + 16 * x + 8 * g);
+#pragma unroll
+              for (int pt = 0; pt < PARTS; ++pt) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, pf[pt], o[d], 0, 0, 0);
+            }
+          } else {
+            // a value that is NaN reaches the rows that read it and no other (its weight of zero would make NaN of the others too): it
+            // is left out of the product, and a second product counts, for every row and dim, the NaN that the row reads
+            float read[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) read[j] = reads(c, 8 * x + j) ? 1.f : 0.f;
+            const bf16x8 rf = to_bf16x8(read);
+#pragma unroll
+            for (int d = 0; d < DB; ++d) {
+              const bf16x8 vf = *reinterpret_cast<const bf16x8*>(Vb + min(32 * d + col, DH - 1) * VROW + 32 * c + 16 * x + 8 * g);
+              float clean[8], bad[8];
+#pragma unroll
+              for (int j = 0; j < 8; ++j) {
+                const float v = static_cast<float>(vf[j]);
+                clean[j] = v == v ? v : 0.f;
+                bad[j] = v == v ? 0.f : 1.f;
+              }
+              const bf16x8 cf = to_bf16x8(clean);
+#pragma unroll
+              for (int pt = 0; pt < PARTS; ++pt) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(cf, pf[pt], o[d], 0, 0, 0);
+              const floatx16 n = __builtin_amdgcn_mfma_f32_32x32x16_bf16(to_bf16x8(bad), rf, zero16, 0, 0, 0);
+#pragma unroll
+              for (int i = 0; i < 16; ++i) o[d][i] = n[i] > 0.5f ? NAN : o[d][i];
+            }
+          }
+        }
+    }
+    __syncthreads();
+  }
+  l_run += other_half(l_run);
+
+  if constexpr (KG > 1) {
+    // the other key groups hand maxima, sums and weighted values to the first, lane to lane; the tiles in LDS are done with
+    if (kg > 0) {
+      float* join = reinterpret_cast<float*>(smem) + ((kg - 1) * THREADS + t) * JOIN;
+      join[0] = m_run;
+      join[1] = l_run;
+#pragma unroll
+      for (int d = 0; d < DB; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) join[2 + 16 * d + i] = o[d][i];
+    }
+    __syncthreads();
+    if (kg > 0) return;
+#pragma unroll
+    for (int k = 0; k < KG - 1; ++k) {
+      const float* join = reinterpret_cast<const float*>(smem) + (k * THREADS + t) * JOIN;
+      const float m_new = fmaxf(m_run, join[0]);
+      const float f0 = __builtin_amdgcn_exp2f(m_run - m_new), f1 = __builtin_amdgcn_exp2f(join[0] - m_new);
+      l_run = l_run * f0 + join[1] * f1;
+      m_run = m_new;
+#pragma unroll
+      for (int d = 0; d < DB; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[d][i] = o[d][i] * f0 + join[2 + 16 * d + i] * f1;
+    }
+  }
+  if (row_ok) {
+    if (a.sink) l_run += __builtin_amdgcn_exp2f((a.sink_at ? a.sink_at[h] : 0.f) * LOG2E - m_run);
+    const float inv = l_run == 0.f ? 0.f : 1.0f / l_run;      // (a row that reads nothing: zeros)
+    const size_t at = static_cast<size_t>(row0 + my_row) * a.ldo + h * DH;
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        const int dim = 32 * d + 8 * x + 4 * g;
+        if (dim < DH) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const float r = o[d][4 * x + j] * inv;
+            if (PARTS == 1) static_cast<bf16_t*>(a.out)[at + dim + j] = from_float<bf16_t>(r);
+            else static_cast<float*>(a.out)[at + dim + j] = r;
+          }
+        }
+      }
+  }
+}
+
+template <int DH16, int PARTS, int RG, int KG>
+static int launch(const Args& a, int n_tiles, hipStream_t stream) {
+  constexpr int DH = DH16 * 16, DB = (DH + 31) / 32;
+  constexpr int TILES = 2 * KG * (64 * (DH + 8) + DH * 72) * 2, JOIN = (KG - 1) * 64 * RG * (2 + 16 * DB) * 4;
+  constexpr int BYTES = (TILES > JOIN ? TILES : JOIN) + 2 * KG * (4 + RG) * 4;
+  static_assert(BYTES <= 160 * 1024, "LDS");
+  auto* fn = &kernel<DH16, PARTS, RG, KG>;
+  if (BYTES > 64 * 1024) {
+    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(fn), hipFuncAttributeMaxDynamicSharedMemorySize, BYTES);
+    if (e != hipSuccess) return static_cast<int>(e);
+  }
+  fn<<<dim3(a.H, n_tiles * (4 / RG)), 64 * RG * KG, BYTES, stream>>>(a);
+  return 0;
+}
+
+template <int DH16, int PARTS>
+static int by_shape(const Args& a, int n_tiles, int rows, int groups, hipStream_t stream) {
+  if (rows == 4 && groups == 1) return launch<DH16, PARTS, 4, 1>(a, n_tiles, stream);
+  if constexpr (DH16 <= 8) {
+    if (rows == 4 && groups == 2) return launch<DH16, PARTS, 4, 2>(a, n_tiles, stream);
+    if (rows == 2 && groups == 2) return launch<DH16, PARTS, 2, 2>(a, n_tiles, stream);
+  }
+  return DN_ERR_SHAPE;
+}
+
+template <int PARTS>
+static int by_dim(const Args& a, int n_tiles, int dh, int rows, int groups, hipStream_t stream) {
+  switch (dh / 16) {
+#define DN_DIM(N) case N: return by_shape<N, PARTS>(a, n_tiles, rows, groups, stream);
+    DN_DIM(1) DN_DIM(2) DN_DIM(3) DN_DIM(4) DN_DIM(5) DN_DIM(6) DN_DIM(7) DN_DIM(8)
+    DN_DIM(9) DN_DIM(10) DN_DIM(11) DN_DIM(12) DN_DIM(13) DN_DIM(14) DN_DIM(15) DN_DIM(16)
+#undef DN_DIM
+  }
+  return DN_ERR_SHAPE;
+}
+}  // namespace portions8
+
+extern "C" int dn_attention8_portions(const void* q, int ldq, void* out, int ldo, const void* k_pool, const void* v_pool,
+                                      const float* k_scale, const float* v_scale, int n_pages, const int32_t* block_tables, int max_blocks,
+                                      const int32_t* tile_seq, const int32_t* tile_row0, const int32_t* tile_nrows,
+                                      const int32_t* tile_pos0, int n_tiles, int rows, int groups, int H, int Hkv, int dh, int page_size,
+                                      float scale, int window, int keep, int sink, const float* sink_at, float cap, int dtype,
+                                      hipStream_t stream) {
+  if (dh < 16 || dh > 256 || dh % 16 != 0 || Hkv < 1 || H % Hkv != 0 || page_size < 16 || page_size % 16 != 0 || !(scale > 0.f) ||
+      window < 0 || keep < 0 || (keep > 0 && window == 0) || !(cap >= 0.f) || ldq % 8 != 0)
+    return DN_ERR_SHAPE;
+  if (dtype != DN_F32 && dtype != DN_BF16) return DN_ERR_DTYPE;
+  if (n_tiles == 0) return 0;
+  const portions8::Args a = {q, out, static_cast<const uint8_t*>(k_pool), static_cast<const uint8_t*>(v_pool), k_scale, v_scale,
+                             block_tables, tile_seq, tile_row0, tile_nrows, tile_pos0, sink_at, ldq, ldo, n_pages, max_blocks, H, Hkv,
+                             page_size, window, keep, sink, scale, cap};
+  const int rc = dtype == DN_BF16 ? portions8::by_dim<1>(a, n_tiles, dh, rows, groups, stream)
+                                  : portions8::by_dim<3>(a, n_tiles, dh, rows, groups, stream);
+  return rc != 0 ? rc : dn_launch_status();
+}

@@ -180,6 +180,7 @@ def _declare(name, lib):
         "cache8": {
             "dn_kv_append8": [P, I, I, I, P, P, P, P, P, I, P, P, I, I, F, I, I, P, I, I, I, I, I, I, P],
             "dn_attention8_single": [P, I, P, I, P, P, P, P, I, P, I, P, P, P, I, P, I, I, I, I, I, I, F, I, I, I, P, F, I, P],
+            "dn_attention8_portions": [P, I, P, I, P, P, P, P, I, P, I, P, P, P, P, I, I, I, I, I, I, I, F, I, I, I, P, F, I, P],
             "dn_attention8": [P, I, P, I, P, P, P, P, I, P, I, P, P, P, P, I, I, I, I, I, F, I, I, I, P, F, I, P],
         },
         "sampling": {
@@ -958,6 +959,11 @@ def _single8_shape(n_tiles, n_heads, Hkv, dh, max_context, window, keep_first):
     return waves, n_splits
 
 
+def _portions8_shape(n_tiles, n_heads, dh):
+    """-> (groups of 32 rows, groups of keys) of a workgroup of the portions' kernel."""
+    return 4, 1
+
+
 def attention8(q, out, k_pool, v_pool, k_scale, v_scale, block_tables, tiles, n_heads, scale, window=0, tiles_wide=None,
                single_rows=False, max_context=0, sink=False, keep_first=0, softcap=0.0):
     """`attention` over a cache in 8 bits as `kv_append8` fills it (that function has the layout of pools and scales): causal attention of
@@ -1003,6 +1009,19 @@ def attention8(q, out, k_pool, v_pool, k_scale, v_scale, block_tables, tiles, n_
                 n_splits, waves, n_heads, Hkv, dh, ps, float(scale), int(window), keep_first, int(sink), _ptr(sink_at), float(softcap),
                 _CODE[q.dtype], _stream()), "attention8 (single rows)")
             return out
+    # (the portions' kernel takes the largest score for the largest product: a scale that is not positive goes the plain way)
+    if aligned and tiles_wide is not None and scale > 0 and ldq % 8 == 0 and q.data_ptr() % 16 == 0:
+        _dev(tiles_wide, "tiles_wide", _I32, 2)
+        _need(tiles_wide.is_contiguous() and tiles_wide.shape[0] == 4, "attention8: tiles_wide")
+        n_wide = tiles_wide.shape[1]
+        rows, groups = _portions8_shape(n_wide, n_heads, dh)
+        base = tiles_wide.data_ptr()
+        _ok(_lib("cache8").dn_attention8_portions(
+            q.data_ptr(), ldq, out.data_ptr(), ldo, k_pool.data_ptr(), v_pool.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
+            n_pages, block_tables.data_ptr(), block_tables.shape[1], base, base + 4 * n_wide, base + 8 * n_wide, base + 12 * n_wide, n_wide,
+            rows, groups, n_heads, Hkv, dh, ps, float(scale), int(window), keep_first, int(sink), _ptr(sink_at), float(softcap),
+            _CODE[q.dtype], _stream()), "attention8 (portions)")
+        return out
     _ok(_lib("cache8").dn_attention8(
         q.data_ptr(), ldq, out.data_ptr(), ldo, k_pool.data_ptr(), v_pool.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), n_pages,
         block_tables.data_ptr(), block_tables.shape[1], base, base + 4 * n_tiles, base + 8 * n_tiles, base + 12 * n_tiles, n_tiles, n_heads,
