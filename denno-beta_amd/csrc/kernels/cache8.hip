@@ -7,7 +7,8 @@
 // append: a step's queries and keys turned by their positions, keys and values to the pages
 // =======================================================================================
 namespace append {
-constexpr int THREADS = 256;
+constexpr int ANY_TASKS = 4;     // tasks of a workgroup of the kernel for any size, one a wave
+constexpr int HEADS = 4;         // heads of a workgroup of the other, one a wave
 constexpr int CHUNK = 16;        // rows whose cos and sin lie in LDS at a time
 constexpr int SCALE_MIN = -117;  // the least exponent of a scale: its smallest number, 2^-9, is then 2^-126, a normal 32-bit one
 
@@ -37,7 +38,7 @@ __device__ __forceinline__ void sin_cos(double a, double& s, double& c) {
   p = fma(p, z, 1.0 / 24.0);
   p = fma(p, z, -0.5);
   const double cr = fma(p, z, 1.0);
-  const long long q = static_cast<long long>(k);
+  const int q = static_cast<int>(k - 4.0 * floor(k * 0.25));
   s = (q & 1) ? cr : sr;
   c = (q & 1) ? sr : cr;
   if (q & 2) s = -s;
@@ -75,69 +76,77 @@ __device__ __forceinline__ uint8_t number_of(float y, float unit) {
 }
 __device__ __forceinline__ float value_of(uint8_t b) { return __builtin_amdgcn_cvt_f32_fp8(static_cast<int>(b), 0); }
 
-// A workgroup takes the rows of one page (a row in whose page the row before does not stand begins such a run) and four
-// tasks of these rows, one a wave: a key head, a value head, a query head.
-template <typename T>
-__global__ __launch_bounds__(THREADS) void kernel(const T* __restrict__ src, int ld, int k_col, int v_col,
-                                                  const int32_t* __restrict__ slot_map, uint8_t* __restrict__ k_pool,
-                                                  uint8_t* __restrict__ v_pool, float* __restrict__ k_scale, float* __restrict__ v_scale,
-                                                  int n_pages, const int32_t* __restrict__ positions, const float* __restrict__ freq,
-                                                  int dims, int halves, float mag, int q_col, int n_heads, T* q_out, int ldq, int rows,
-                                                  int Hkv, int dh, int page_size) {
-  extern __shared__ double turn[];      // [CHUNK][dims / 2] pairs (cos, sin)
-  const int t0 = blockIdx.x;
-  auto page_of = [&](int t) {
-    const int s = slot_map[t];
-    const int p = s < 0 ? -1 : s / page_size;
-    return p < n_pages ? p : -1;
-  };
-  const int page = page_of(t0);
-  if (page >= 0 && t0 > 0 && page_of(t0 - 1) == page) return;      // the whole workgroup: this row is another run's
-  const int wave = threadIdx.x / 64, lane = threadIdx.x % 64;
-  // the run's rows t0 .. t0 + n (a row without a page is a run of its own)
+struct Args {
+  const void* src;
+  const int32_t* slot_map;
+  uint8_t *k_pool, *v_pool;
+  float *k_scale, *v_scale;
+  const int32_t* positions;
+  const float* freq;
+  void* q_out;
+  int ld, k_col, v_col, n_pages, dims, halves, q_col, n_heads, ldq, rows, Hkv, dh, page_size, page_shift;      // page_shift: -1 if page_size is no power of two
+  float mag;
+  // (a division by a number known only at run time is some twenty-five instructions)
+  __device__ __forceinline__ int over_page(int slot) const { return page_shift >= 0 ? slot >> page_shift : slot / page_size; }
+};
+
+// the page of row t, -1: none
+__device__ __forceinline__ int page_of(const Args& a, int t) {
+  const int s = a.slot_map[t];
+  const int p = s < 0 ? -1 : a.over_page(s);
+  return p < a.n_pages ? p : -1;
+}
+
+// how many rows from t0 on stand in `page`
+__device__ __forceinline__ int rows_in_page(const Args& a, int t0, int page, int lane) {
   int n = 1;
-  if (page >= 0) {
-    for (;;) {
-      const int t = t0 + n + lane;
-      const bool same = t < rows && page_of(min(t, rows - 1)) == page;
-      const uint64_t other = ~__builtin_amdgcn_ballot_w64(same);
-      const int more = other ? __builtin_ctzll(other) : 64;
-      n += more;
-      if (more < 64) break;
-    }
+  for (;;) {
+    const int t = t0 + n + lane;
+    const bool same = t < a.rows && page_of(a, min(t, a.rows - 1)) == page;
+    const uint64_t other = ~__builtin_amdgcn_ballot_w64(same);
+    const int more = other ? __builtin_ctzll(other) : 64;
+    n += more;
+    if (more < 64) return n;
   }
-  const int half = dims / 2;
-  const int task = blockIdx.y * (THREADS / 64) + wave;
-  const int kind = task < Hkv ? 0 : task < 2 * Hkv ? 1 : task < 2 * Hkv + n_heads ? 2 : 3;
+}
+
+// Every size and any order of a page's rows.  A workgroup takes the rows t0 .. t0 + n of one page and four tasks of these rows, one a
+// wave: a key head, a value head, a query head; a number, or a pair of them, at a time.
+template <typename T>
+__device__ __forceinline__ void any_size(const Args& a, double* turn, int t0, int n, int page, int first_task, int wave, int lane) {
+  const int half = a.dims / 2, dh = a.dh, page_size = a.page_size, Hkv = a.Hkv;
+  const T* src = static_cast<const T*>(a.src);
+  const int task = first_task + wave;
+  const int kind = task < Hkv ? 0 : task < 2 * Hkv ? 1 : task < 2 * Hkv + a.n_heads ? 2 : 3;
   const bool idle = kind == 3 || (kind < 2 && page < 0);
   const int head = kind == 0 ? task : kind == 1 ? task - Hkv : task - 2 * Hkv;
-  const int col = (kind == 0 ? k_col : kind == 1 ? v_col : q_col) + head * dh;
+  const int col = (kind == 0 ? a.k_col : kind == 1 ? a.v_col : a.q_col) + head * dh;
   const int turned = kind == 1 ? 0 : half;      // pairs that this task's heads turn
   const int units = turned + dh - 2 * turned;   // a row's units: a pair each, then a number each
   const size_t block = (static_cast<size_t>(max(page, 0)) * Hkv + head) * page_size * dh;
 
   // unit u of row r (of the chunk that begins with row c): its numbers, at entries i and j (j < 0: one number)
-  auto unit = [&](int c, int r, int u, int& i, int& j, double& a, double& b) {
-    const T* x = src + static_cast<size_t>(t0 + c + r) * ld + col;
+  auto unit = [&](int c, int r, int u, int& i, int& j, double& p, double& q) {
+    const T* x = src + static_cast<size_t>(t0 + c + r) * a.ld + col;
     if (u < turned) {
-      i = halves ? u : 2 * u;
-      j = halves ? u + half : 2 * u + 1;
+      i = a.halves ? u : 2 * u;
+      j = a.halves ? u + half : 2 * u + 1;
       const double* cs = turn + (static_cast<size_t>(r) * half + u) * 2;
-      const double p = to_float(x[i]), q = to_float(x[j]);
-      a = (p * cs[0] - q * cs[1]) * mag;
-      b = (q * cs[0] + p * cs[1]) * mag;
+      const double v = to_float(x[i]), w = to_float(x[j]);
+      p = (v * cs[0] - w * cs[1]) * a.mag;
+      q = (w * cs[0] + v * cs[1]) * a.mag;
     } else {
       i = u + turned;
       j = -1;
-      a = to_float(x[i]);
-      b = 0.0;
+      p = to_float(x[i]);
+      q = 0.0;
     }
   };
   auto angles = [&](int c) {      // cos and sin of the chunk's rows, by the whole workgroup
     __syncthreads();
-    for (int x = threadIdx.x; x < min(CHUNK, n - c) * half; x += THREADS) {
+    for (int x = threadIdx.x; x < min(CHUNK, n - c) * half; x += blockDim.x) {
       double s, k;
-      sin_cos(static_cast<double>(positions[t0 + c + x / half]) * static_cast<double>(freq[x % half]), s, k);
+      sin_cos(static_cast<double>(a.positions[t0 + c + x / half]) * static_cast<double>(a.freq[x % half]), s, k);
       turn[2 * x] = k;
       turn[2 * x + 1] = s;
     }
@@ -153,27 +162,27 @@ __global__ __launch_bounds__(THREADS) void kernel(const T* __restrict__ src, int
     const int m = min(CHUNK, n - c) * units;
     for (int x = lane; x < m; x += 64) {
       int i, j;
-      double a, b;
-      unit(c, x / units, x % units, i, j, a, b);
+      double p, q;
+      unit(c, x / units, x % units, i, j, p, q);
       if (kind == 2) {
-        T* o = q_out + static_cast<size_t>(t0 + c + x / units) * ldq + head * dh;
-        o[i] = from_float<T>(static_cast<float>(a));
-        if (j >= 0) o[j] = from_float<T>(static_cast<float>(b));
+        T* o = static_cast<T*>(a.q_out) + static_cast<size_t>(t0 + c + x / units) * a.ldq + head * dh;
+        o[i] = from_float<T>(static_cast<float>(p));
+        if (j >= 0) o[j] = from_float<T>(static_cast<float>(q));
       } else {
-        const float fa = fabsf(to_odd(a)), fb = fabsf(to_odd(b));
-        top = fmaxf(top, finite(fa) ? fa : 0.f);
-        top = fmaxf(top, finite(fb) ? fb : 0.f);
+        const float fp = fabsf(to_odd(p)), fq = fabsf(to_odd(q));
+        top = fmaxf(top, finite(fp) ? fp : 0.f);
+        top = fmaxf(top, finite(fq) ? fq : 0.f);
       }
     }
     if (kind < 2)
-      for (int r = 0; r < min(CHUNK, n - c); ++r) anew = anew || slot_map[t0 + c + r] % page_size == 0;
+      for (int r = 0; r < min(CHUNK, n - c); ++r) anew = anew || a.slot_map[t0 + c + r] % page_size == 0;
   }
   // (every wave of the workgroup has to pass every barrier below, tasks or none)
   const bool writes = !idle && kind < 2;
   float now = 1.f;
+  uint8_t* pool = (kind == 0 ? a.k_pool : a.v_pool) + block;
   if (writes) {
-    uint8_t* pool = (kind == 0 ? k_pool : v_pool) + block;
-    float* scale = (kind == 0 ? k_scale : v_scale) + static_cast<size_t>(page) * Hkv + head;
+    float* scale = (kind == 0 ? a.k_scale : a.v_scale) + static_cast<size_t>(page) * Hkv + head;
     top = wave_max(top);
     const float was = anew ? 0.f : *scale;
     now = fmaxf(power_of_two(scale_exponent(top)), was);
@@ -191,16 +200,380 @@ __global__ __launch_bounds__(THREADS) void kernel(const T* __restrict__ src, int
   for (int c = 0; c < n; c += CHUNK) {
     if (half > 0 && n > CHUNK) angles(c);
     if (!writes) continue;
-    uint8_t* pool = (kind == 0 ? k_pool : v_pool) + block;
     const int m = min(CHUNK, n - c) * units;
     for (int x = lane; x < m; x += 64) {
-      const int r = x / units, place = slot_map[t0 + c + r] % page_size;
+      const int r = x / units, place = a.slot_map[t0 + c + r] % page_size;
       int i, j;
-      double a, b;
-      unit(c, r, x % units, i, j, a, b);
-      pool[kind == 0 ? place * dh + i : i * page_size + place] = number_of(to_odd(a), per);
-      if (j >= 0) pool[kind == 0 ? place * dh + j : j * page_size + place] = number_of(to_odd(b), per);
+      double p, q;
+      unit(c, r, x % units, i, j, p, q);
+      pool[kind == 0 ? place * dh + i : i * page_size + place] = number_of(to_odd(p), per);
+      if (j >= 0) pool[kind == 0 ? place * dh + j : j * page_size + place] = number_of(to_odd(q), per);
     }
+  }
+}
+
+template <typename T>
+__global__ __launch_bounds__(64 * ANY_TASKS) void any_size_kernel(const Args a) {
+  extern __shared__ double turn[];      // [CHUNK][dims / 2] pairs (cos, sin)
+  const int t0 = blockIdx.x, page = page_of(a, t0);
+  if (page >= 0 && t0 > 0 && page_of(a, t0 - 1) == page) return;      // the whole workgroup: this row is another run's
+  const int lane = threadIdx.x % 64;
+  const int n = page >= 0 ? rows_in_page(a, t0, page, lane) : 1;      // (a row without a page is a run of its own)
+  any_size<T>(a, turn, t0, n, page, blockIdx.y * ANY_TASKS, threadIdx.x / 64, lane);
+}
+
+// The sizes of models: heads of a multiple of 8, turned entries likewise, pages of a multiple of 16, rows 16-byte aligned.  What bounds
+// these calls is bytes (portions) or a chain of a few trips to memory (single rows), so numbers move eight at a time, and the
+// angles' sines, some 60 instructions of 64 bits each, are made once per workgroup for the eight heads that it turns.
+//   keys and queries: a lane takes a unit of 8 entries of a row: two runs of four, side by side, or with halves half a turn apart;
+//   values: a lane takes two dims and a block of 16 places, so that a dim's 16 numbers, which lie side by side in the page, leave
+//   in one store; what the page holds in that block already is read beside the rows.
+typedef __attribute__((__vector_size__(4 * sizeof(uint32_t)))) uint32_t u32x4;
+typedef __attribute__((__vector_size__(2 * sizeof(uint32_t)))) uint32_t u32x2;
+typedef __attribute__((__vector_size__(4 * sizeof(float)))) float floatx4;
+
+__device__ __forceinline__ void load4(const bf16_t* p, float* v) {
+  const u32x2 w = *reinterpret_cast<const u32x2*>(p);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] = __uint_as_float((i & 1) ? w[i / 2] & 0xffff0000u : w[i / 2] << 16);
+}
+__device__ __forceinline__ void load4(const float* p, float* v) {
+  const floatx4 w = *reinterpret_cast<const floatx4*>(p);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] = w[i];
+}
+__device__ __forceinline__ void load2(const bf16_t* p, float* v) {
+  const uint32_t w = *reinterpret_cast<const uint32_t*>(p);
+  v[0] = __uint_as_float(w << 16), v[1] = __uint_as_float(w & 0xffff0000u);
+}
+__device__ __forceinline__ void load2(const float* p, float* v) { v[0] = p[0], v[1] = p[1]; }
+__device__ __forceinline__ void store4(bf16_t* p, const float* v) {
+  u32x2 w;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) w[i] = static_cast<uint32_t>(from_float<bf16_t>(v[2 * i]).bits) | static_cast<uint32_t>(from_float<bf16_t>(v[2 * i + 1]).bits) << 16;
+  *reinterpret_cast<u32x2*>(p) = w;
+}
+__device__ __forceinline__ void store4(float* p, const float* v) { *reinterpret_cast<floatx4*>(p) = floatx4{v[0], v[1], v[2], v[3]}; }
+
+// four numbers of a page (number_of), in one word
+__device__ __forceinline__ uint32_t numbers_of(const float* y, float unit) {
+  float f[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    f[i] = y[i] * unit;
+    f[i] = finite(f[i]) ? f[i] : NAN;
+  }
+  return __builtin_amdgcn_cvt_pk_fp8_f32(f[2], f[3], __builtin_amdgcn_cvt_pk_fp8_f32(f[0], f[1], 0, false), true);
+}
+// a word of numbers in a page whose scale grew
+__device__ __forceinline__ uint32_t renumbered(uint32_t w, float ratio) {
+  const float y[4] = {__builtin_amdgcn_cvt_f32_fp8(w, 0), __builtin_amdgcn_cvt_f32_fp8(w, 1), __builtin_amdgcn_cvt_f32_fp8(w, 2), __builtin_amdgcn_cvt_f32_fp8(w, 3)};
+  return numbers_of(y, ratio);
+}
+
+// The angles' sines of rows t0 .. t0 + n, by the whole workgroup.  turn: [rows][4][dims / 8] pairs (cos, sin): pair 4 u + k at [k][u], so
+// that lanes side by side read side by side.
+__device__ __forceinline__ void angles(const Args& a, double* turn, int t0, int n, int wave, int lane) {
+  // (half up to 128: a power of two of threads, the least that holds a row's pairs, takes a row)
+  const int half = a.dims / 2, bits = half > 1 ? 32 - __builtin_clz(half - 1) : 0;
+  const int x = wave * 64 + lane, p = x & ((1 << bits) - 1);
+  if (p < half) {
+    const double f = a.freq[p];
+    for (int r = x >> bits; r < n; r += 64 * HEADS >> bits) {
+      double s, c;
+      sin_cos(static_cast<double>(a.positions[t0 + r]) * f, s, c);
+      double* to = turn + 2 * (r * half + p % 4 * (half / 4) + p / 4);
+      to[0] = c * a.mag;
+      to[1] = s * a.mag;
+    }
+  }
+  __syncthreads();
+}
+
+// A lane's unit u of a row: its two runs of four entries begin at ea and eb.
+template <typename T, bool HALVES>
+struct Unit {
+  int u, ea, eb, half;
+  bool turned;
+  __device__ __forceinline__ Unit(const Args& a, int u_) : u(u_), half(a.dims / 2), turned(u_ < a.dims / 8) {
+    ea = HALVES && turned ? 4 * u : 8 * u;
+    eb = HALVES && turned ? half + 4 * u : 8 * u + 4;
+  }
+  __device__ __forceinline__ void load(const T* row, float* v) const { load4(row + ea, v), load4(row + eb, v + 4); }
+  // turned as row r's angles say, rounded to 32 bits.  KEYS: so that a second rounding to e4m3 is what rounding the 64-bit number would be,
+  // and so that the largest magnitude compares with 1.75 * 2^k as the 64-bit one does.  Either can go wrong only where the 32-bit number
+  // stands on a border itself, and those have zeros in their last 19 bits: there (once in half a million) the last bit is set odd.
+  template <bool KEYS>
+  __device__ __forceinline__ void turn(const double* angles, int r, float* v) const {
+    if (!turned) return;
+    float w[8];
+    bool border = false;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const double* cs = angles + 2 * (r * half + k * (half / 4) + u);
+      const int i = HALVES ? k : 2 * k, j = HALVES ? 4 + k : 2 * k + 1;
+      const double c = cs[0], s = cs[1], p = v[i], q = v[j];
+      w[i] = static_cast<float>(p * c - q * s);
+      w[j] = static_cast<float>(q * c + p * s);
+      if (KEYS) border = border | ((__float_as_uint(w[i]) & 0x7ffffu) == 0) | ((__float_as_uint(w[j]) & 0x7ffffu) == 0);
+    }
+    if (KEYS && __builtin_amdgcn_ballot_w64(border) != 0) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const double* cs = angles + 2 * (r * half + k * (half / 4) + u);
+        const int i = HALVES ? k : 2 * k, j = HALVES ? 4 + k : 2 * k + 1;
+        const double c = cs[0], s = cs[1], p = v[i], q = v[j];
+        w[i] = to_odd(p * c - q * s);
+        w[j] = to_odd(q * c + p * s);
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] = w[k];
+  }
+};
+constexpr int UNITS = 4, KEY_UNITS = 4;      // units of a lane in flight (keys take more registers)
+
+// rows t0 .. t0 + n (n <= UNITS) of the queries
+template <typename T, bool HALVES>
+__device__ __forceinline__ void turn_queries(const Args& a, double* turn, int t0, int n, int wave, int lane) {
+  const int per_row = a.dh / 8, span = 64 / per_row, of = lane / per_row;
+  const Unit<T, HALVES> unit(a, lane % per_row);
+  const T* x = static_cast<const T*>(a.src) + static_cast<size_t>(t0) * a.ld + a.q_col;
+  T* o = static_cast<T*>(a.q_out) + static_cast<size_t>(t0) * a.ldq;
+  float v[UNITS][8];
+  auto load = [&](int head) {
+#pragma unroll
+    for (int i = 0; i < UNITS; ++i)
+      unit.load(x + static_cast<size_t>(min(i, n - 1)) * a.ld + head * a.dh, v[i]);
+  };
+  const int first = of < span ? wave * span + of : a.n_heads;
+  load(min(first, a.n_heads - 1));
+  angles(a, turn, t0, n, wave, lane);
+  for (int head = first; head < a.n_heads; head += HEADS * span) {
+    if (head != first) load(head);
+#pragma unroll
+    for (int i = 0; i < UNITS; ++i) {
+      if (i < n) {
+        unit.template turn<false>(turn, i, v[i]);
+        T* to = o + static_cast<size_t>(i) * a.ldq + head * a.dh;
+        store4(to + unit.ea, v[i]);
+        store4(to + unit.eb, v[i] + 4);
+      }
+      __builtin_amdgcn_sched_barrier(0);      // (one unit's 64-bit numbers at a time)
+    }
+  }
+}
+
+// The rows t0 .. t0 + n, which stand in one page, of eight key heads (group < ceil(Hkv / 8)) or value heads (the groups behind).
+template <typename T, bool HALVES>
+__device__ __forceinline__ void run_of_rows(const Args& a, double* turn, int* row_in, int group, int t0, int n, int page, int place0, bool odd, int wave,
+                                            int lane) {
+  const int ps = a.page_size, dh = a.dh, kv_groups = (a.Hkv + HEADS - 1) / HEADS;
+  const bool values = group >= kv_groups;
+  const int head = (values ? group - kv_groups : group) * HEADS + wave;
+  if (odd) {      // (the same for every wave of the workgroup) rows in another order than their places': the row of every place, -1: none
+    for (int i = threadIdx.x; i < ps; i += 64 * HEADS) row_in[i] = -1;
+    __syncthreads();
+    for (int r = threadIdx.x; r < n; r += 64 * HEADS) row_in[a.slot_map[t0 + r] - page * ps] = r;
+    __syncthreads();
+  }
+  auto row_at = [&](int place) {
+    if (odd) return row_in[place];
+    return place >= place0 && place < place0 + n ? place - place0 : -1;
+  };
+  const T* src = static_cast<const T*>(a.src) + static_cast<size_t>(t0) * a.ld;
+  const bool anew = odd ? row_in[0] >= 0 : place0 == 0;
+
+  if (values) {
+    if (head >= a.Hkv) return;      // (no barrier in this part)
+    const T* x = src + a.v_col + head * dh;
+    uint8_t* pool = a.v_pool + (static_cast<size_t>(page) * a.Hkv + head) * ps * dh;
+    float* scale = a.v_scale + static_cast<size_t>(page) * a.Hkv + head;
+    const float was = anew ? 0.f : *scale;
+    if (n == 1 && !anew) {
+      // one row, as a decode step brings it: unless the scale grows, its bytes are all that is stored
+      float y[4][2], top = 0.f;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int d = 2 * lane + 128 * i;
+        y[i][0] = y[i][1] = 0.f;
+        if (d < dh) load2(x + d, y[i]);
+#pragma unroll
+        for (int j = 0; j < 2; ++j) top = fmaxf(top, finite(y[i][j]) ? fabsf(y[i][j]) : 0.f);
+      }
+      top = wave_max(top);
+      const float now = fmaxf(power_of_two(scale_exponent(top)), was);
+      if (now == was) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int d = 2 * lane + 128 * i;
+          if (d < dh) {
+            pool[static_cast<size_t>(d) * ps + place0] = number_of(y[i][0], 1.0f / now);
+            pool[static_cast<size_t>(d + 1) * ps + place0] = number_of(y[i][1], 1.0f / now);
+          }
+        }
+        return;
+      }
+    }
+    // a lane's unit x: a pair of dims and a block of 16 places
+    const int pairs = dh / 2, units = pairs * (ps / 16);
+    const int b0 = odd ? 0 : place0 / 16, b1 = odd ? ps / 16 - 1 : (place0 + n - 1) / 16;      // the blocks that rows bring something to
+    const bool once = units <= 64;      // (rows and page stay in registers)
+    float y[16][2];
+    uint32_t mask[4];      // the bytes of the block that rows bring
+    u32x4 held[2];
+    auto load = [&](int d, int b) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        // (never a conditional load, here and below: sixteen branches cost more than sixteen loads of a row already asked for; 10.1 -> 7.1 us)
+        const int r = row_at(16 * b + i);
+        load2(x + static_cast<size_t>(max(r, 0)) * a.ld + d, y[i]);
+        if (r < 0) y[i][0] = y[i][1] = 0.f;
+        const uint32_t byte = r >= 0 ? 0xffu << (8 * (i % 4)) : 0u;
+        mask[i / 4] = i % 4 == 0 ? byte : mask[i / 4] | byte;
+      }
+    };
+    auto load_held = [&](int d, int b) {
+#pragma unroll
+      for (int j = 0; j < 2; ++j) held[j] = anew ? u32x4{0u, 0u, 0u, 0u} : *reinterpret_cast<const u32x4*>(pool + static_cast<size_t>(d + j) * ps + 16 * b);
+    };
+    float top = 0.f;
+    for (int i = lane; i < units; i += 64) {
+      const int b = i / pairs, d = 2 * (i - b * pairs);
+      if (once) load_held(d, b);
+      if (once || (b >= b0 && b <= b1)) load(d, b);
+      if (b >= b0 && b <= b1) {
+#pragma unroll
+        for (int k = 0; k < 16; ++k)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) top = fmaxf(top, finite(y[k][j]) ? fabsf(y[k][j]) : 0.f);
+      }
+    }
+    top = wave_max(top);
+    const float now = fmaxf(power_of_two(scale_exponent(top)), was), per = 1.0f / now, ratio = was / now;
+    const bool grown = now != was;
+    if (grown && lane == 0) *scale = now;
+    for (int i = lane; i < units; i += 64) {
+      const int b = i / pairs, d = 2 * (i - b * pairs);
+      if (!grown && (b < b0 || b > b1)) continue;
+      if (!once) load_held(d, b), load(d, b);
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        u32x4 w;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const float z[4] = {y[4 * q][j], y[4 * q + 1][j], y[4 * q + 2][j], y[4 * q + 3][j]};
+          const uint32_t old = grown && !anew ? renumbered(held[j][q], ratio) : held[j][q];
+          w[q] = (numbers_of(z, per) & mask[q]) | (old & ~mask[q]);
+        }
+        *reinterpret_cast<u32x4*>(pool + static_cast<size_t>(d + j) * ps + 16 * b) = w;
+      }
+    }
+    return;
+  }
+
+  // keys: `span` rows at a time
+  const int per_row = dh / 8, span = 64 / per_row, of = lane / per_row;
+  const Unit<T, HALVES> unit(a, lane % per_row);
+  const int end = of < span && head < a.Hkv ? n : 0;      // (a lane without work has no rows)
+  const T* x = src + a.k_col + min(head, a.Hkv - 1) * dh;
+  float v[KEY_UNITS][8];
+  auto load = [&](int r0) {
+#pragma unroll
+    for (int i = 0; i < KEY_UNITS; ++i) unit.load(x + static_cast<size_t>(min(r0 + of + i * span, n - 1)) * a.ld, v[i]);
+  };
+  auto turn_all = [&](int r0) {
+#pragma unroll
+    for (int i = 0; i < KEY_UNITS; ++i) {
+      if (r0 + of + i * span < end) unit.template turn<true>(turn, r0 + of + i * span, v[i]);
+      __builtin_amdgcn_sched_barrier(0);      // (one unit's 64-bit numbers at a time)
+    }
+  };
+  load(0);
+  float* scale = a.k_scale + static_cast<size_t>(page) * a.Hkv + head;
+  const float was = anew || head >= a.Hkv ? 0.f : *scale;
+  if (a.dims > 0) angles(a, turn, t0, n, wave, lane);
+  if (head >= a.Hkv) return;      // (no barrier below)
+  uint8_t* pool = a.k_pool + (static_cast<size_t>(page) * a.Hkv + head) * ps * dh;
+  const bool once = n <= KEY_UNITS * span;
+  float top = 0.f;
+  for (int r0 = 0; r0 < n; r0 += KEY_UNITS * span) {
+    if (r0 > 0) load(r0);
+    turn_all(r0);
+#pragma unroll
+    for (int i = 0; i < KEY_UNITS; ++i)
+      if (r0 + of + i * span < end) {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) top = fmaxf(top, finite(v[i][k]) ? fabsf(v[i][k]) : 0.f);
+      }
+  }
+  top = wave_max(top);
+  const float now = fmaxf(power_of_two(scale_exponent(top)), was), per = 1.0f / now;
+  if (now != was) {      // what the page holds in other places
+    if (lane == 0) *scale = now;
+    const float ratio = was / now;
+    for (int place = of; place < ps && of < span; place += span) {
+      if (row_at(place) >= 0) continue;
+      u32x2* at = reinterpret_cast<u32x2*>(pool + static_cast<size_t>(place) * dh + unit.u * 8);
+      u32x2 w = {0u, 0u};
+      if (!anew) w = *at, w = u32x2{renumbered(w[0], ratio), renumbered(w[1], ratio)};
+      *at = w;
+    }
+  }
+  for (int r0 = 0; r0 < n; r0 += KEY_UNITS * span) {
+    if (!once) load(r0), turn_all(r0);      // (read a second time, out of the caches)
+#pragma unroll
+    for (int i = 0; i < KEY_UNITS; ++i) {
+      const int r = r0 + of + i * span;
+      if (r < end) {
+        uint8_t* to = pool + static_cast<size_t>(odd ? a.slot_map[t0 + r] - page * ps : place0 + r) * dh;
+        *reinterpret_cast<uint32_t*>(to + unit.ea) = numbers_of(v[i], per);
+        *reinterpret_cast<uint32_t*>(to + unit.eb) = numbers_of(v[i] + 4, per);
+      }
+    }
+  }
+}
+
+// The first workgroups take Q rows of queries each.  Of the others, each looks for the runs of rows in one page that begin among its R rows.
+// (A workgroup that finds none costs 2.7 ns of the launch all the same: with one for every row, 2,136 rows of 32 + 8 + 8 heads of
+// 128 took 68 us.)
+template <typename T, bool HALVES>
+__global__ __launch_bounds__(64 * HEADS) __attribute__((amdgpu_waves_per_eu(3))) void kernel(const Args a, int q_blocks, int Q, int R) {
+  extern __shared__ double turn[];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64;
+  if (static_cast<int>(blockIdx.x) < q_blocks) {
+    const int t0 = blockIdx.x * Q;
+    turn_queries<T, HALVES>(a, turn, t0, min(Q, a.rows - t0), wave, lane);
+    return;
+  }
+  int* const row_in = reinterpret_cast<int*>(turn + static_cast<size_t>(a.page_size) * a.dims);
+  const int groups = 2 * ((a.Hkv + HEADS - 1) / HEADS), group = (blockIdx.x - q_blocks) % groups, block = (blockIdx.x - q_blocks) / groups;
+  const int ps = a.page_size, end = min(a.rows, (block + 1) * R);
+  for (int t0 = block * R; t0 < end;) {
+    // lane i: the slot of row t0 - 1 + i (one load for the row before, the run's length and its places)
+    const int t = t0 - 1 + lane;
+    const int slot = t >= 0 && t < a.rows ? a.slot_map[t] : -1;
+    const int its = a.over_page(slot), its_page = slot < 0 || its >= a.n_pages ? -1 : its;
+    const int page = __builtin_amdgcn_readlane(its_page, 1), place0 = __builtin_amdgcn_readlane(slot - its * ps, 1);
+    if (page < 0) {
+      ++t0;
+      continue;
+    }
+    const uint64_t same = __builtin_amdgcn_ballot_w64(its_page == page);
+    int n = 1 + __builtin_ctzll(~(same >> 2));      // (at most 63: the two bits shifted in are zeros)
+    if (same & 1) {                                 // the row before stands in this page too: this is the rest of another workgroup's run
+      t0 += n;
+      continue;
+    }
+    if (n == 63) n = rows_in_page(a, t0, page, lane);
+    // rows in another order than their places'
+    bool odd = n > ps - place0 || (lane >= 1 && lane <= n && slot != page * ps + place0 + lane - 1);
+    for (int r = 63 + lane; r < n; r += 64) odd = odd || a.slot_map[t0 + r] != page * ps + place0 + r;
+    odd = __builtin_amdgcn_ballot_w64(odd) != 0;
+    // (more rows than places have a slot twice, which is not allowed: those behind are left out, so that what LDS holds suffices)
+    run_of_rows<T, HALVES>(a, turn, row_in, group, t0, min(n, ps), page, place0, odd, wave, lane);
+    t0 += n;
+    if (t0 < end) __syncthreads();      // (the next run's angles and places take these ones' room)
   }
 }
 }  // namespace append
@@ -212,16 +585,40 @@ extern "C" int dn_kv_append8(const void* src, int ld, int k_col, int v_col, cons
   if (dims < 0 || dims % 2 != 0 || dims > dh || dh < 1 || dh > 256 || page_size < 1 || Hkv < 1 || n_heads < 0 || n_pages < 1) return DN_ERR_SHAPE;
   if (dtype != DN_F32 && dtype != DN_BF16) return DN_ERR_DTYPE;
   if (T == 0) return 0;
-  const dim3 grid(T, (2 * Hkv + n_heads + 3) / 4);
-  const size_t lds = static_cast<size_t>(append::CHUNK) * dims * sizeof(double);
-#define DN_APPEND(TYPE)                                                                                                          \
-  append::kernel<TYPE><<<grid, append::THREADS, lds, stream>>>(                                                                  \
-      static_cast<const TYPE*>(src), ld, k_col, v_col, slot_map, static_cast<uint8_t*>(k_pool), static_cast<uint8_t*>(v_pool),   \
-      k_scale, v_scale, n_pages, positions, freq, dims, halves, mag, q_col, n_heads, static_cast<TYPE*>(q_out), ldq, T, Hkv, dh, \
-      page_size)
-  if (dtype == DN_F32) DN_APPEND(float);
-  else DN_APPEND(bf16_t);
+  int page_shift = 0;
+  while ((1 << page_shift) < page_size) ++page_shift;
+  if ((1 << page_shift) != page_size) page_shift = -1;
+  const append::Args a = {src, slot_map, static_cast<uint8_t*>(k_pool), static_cast<uint8_t*>(v_pool), k_scale, v_scale, positions, freq, q_out,
+                          ld, k_col, v_col, n_pages, dims, halves, q_col, n_heads, ldq, T, Hkv, dh, page_size, page_shift, mag};
+  // rows of a page in LDS at a time; the kernel for other sizes takes them 16 at a time, whatever the page
+  const size_t lds = static_cast<size_t>(append::CHUNK) * dims * sizeof(double), lds_page = static_cast<size_t>(page_size) * (dims * sizeof(double) + sizeof(int));
+  const int size = dtype == DN_F32 ? 4 : 2;
+  auto whole = [&](const void* p, int stride, int col) {
+    return (reinterpret_cast<uintptr_t>(p) + static_cast<size_t>(col) * size) % 16 == 0 && static_cast<size_t>(stride) * size % 16 == 0;
+  };
+  const bool fast = dh % 8 == 0 && dims % 8 == 0 && page_size % 16 == 0 && lds_page <= 64 * 1024 && whole(src, ld, k_col) && whole(src, ld, v_col) &&
+                    (n_heads == 0 || (whole(src, ld, q_col) && whole(q_out, ldq, 0))) && reinterpret_cast<uintptr_t>(k_pool) % 16 == 0 &&
+                    reinterpret_cast<uintptr_t>(v_pool) % 16 == 0;
+  if (fast) {
+    // a workgroup for every row as long as that makes no more than 1,024, else for 2, 4, 8, ... rows
+    const int groups = 2 * ((Hkv + append::HEADS - 1) / append::HEADS), Q = T <= 512 ? 1 : append::UNITS, q_blocks = n_heads > 0 ? (T + Q - 1) / Q : 0;
+    int R = 1;
+    while (static_cast<long>((T + R - 1) / R) * groups > 1024 && R < T) R *= 2;
+    const dim3 grid(q_blocks + (T + R - 1) / R * groups);
+#define DN_APPEND(TYPE, HALVES) append::kernel<TYPE, HALVES><<<grid, 64 * append::HEADS, lds_page, stream>>>(a, q_blocks, Q, R)
+    if (dtype == DN_F32) {
+      if (halves) DN_APPEND(float, true);
+      else DN_APPEND(float, false);
+    } else {
+      if (halves) DN_APPEND(bf16_t, true);
+      else DN_APPEND(bf16_t, false);
+    }
 #undef DN_APPEND
+  } else {
+    const dim3 grid(T, (2 * Hkv + n_heads + append::ANY_TASKS - 1) / append::ANY_TASKS);
+    if (dtype == DN_F32) append::any_size_kernel<float><<<grid, 64 * append::ANY_TASKS, lds, stream>>>(a);
+    else append::any_size_kernel<bf16_t><<<grid, 64 * append::ANY_TASKS, lds, stream>>>(a);
+  }
   return dn_launch_status();
 }
 

@@ -179,6 +179,31 @@ def test_append_token_by_token_and_at_once():
         assert bool(((a - b).abs() <= 2.0 ** -9).all()) and bool((a == b)[a.abs() >= 2.0 ** -5].all())
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("dh,ps,turn,dims", [(64, 16, "pairs", 64), (128, 32, "halves", 96), (48, 16, "none", 0)])
+def test_append_rows_of_a_page_in_any_order(dtype, dh, ps, turn, dims):
+    """The rows of a page stand side by side, but not in the order of their places; the pages before and behind are in order."""
+    gen = torch.Generator().manual_seed(6)
+    H, hkv = 10, 5
+    slots = [3 * ps + i for i in range(ps)] + [ps + i for i in (5, 4, 9, 0, 2)] + [2 * ps + 7 - i for i in range(4)] + [i for i in range(1, 9)]
+    T = len(slots)
+    src = (torch.randn(T, (H + 2 * hkv) * dh, generator=gen) * torch.exp(torch.randn(T, 1, generator=gen))).to(dtype)
+    pools = random_pools(5, hkv, ps, dh, gen)
+    kw = {}
+    if dims:
+        kw = dict(positions=i32(range(100, 100 + T)), freq=(10000.0 ** (-torch.arange(dims // 2).double() * 2 / dims)).float(), halves=turn == "halves",
+                  q_col=0, n_heads=H)
+    want, q_want = [p.clone() for p in pools], torch.zeros(T, H * dh, dtype=dtype)
+    R.kv_append8(src, H * dh, (H + hkv) * dh, i32(slots), *want, **dict(kw, **({"q_out": q_want} if kw else {})))
+    got, q_got = [p.to(DEV) for p in pools], torch.zeros(T, H * dh, dtype=dtype, device=DEV)
+    ops().kv_append8(src.to(DEV), H * dh, (H + hkv) * dh, i32(slots).to(DEV), *got,
+                     **{k: v.to(DEV) if isinstance(v, torch.Tensor) else v for k, v in kw.items()}, **({"q_out": q_got} if kw else {}))
+    for name, a, b in zip(("keys", "values", "key scales", "value scales"), got, want):
+        assert same(a, b), name
+    if kw:
+        assert bool(((q_got.cpu().double() - q_want.double()).abs() <= 2 * (HALF[dtype] + 2.0 ** -24) * q_want.double().abs() + 1e-300).all())
+
+
 # -- attention -----------------------------------------------------------------------------------------------------------------
 
 def attention_case(seq_lens, new_rows, H, hkv, dh, ps, dtype, seed=0, q_scale=1.0, window=0, keep=0):
