@@ -876,7 +876,15 @@ def attention(q, out, k_pool, v_pool, block_tables, tiles, n_heads, scale, windo
 
 def _pools8(k_pool, v_pool, k_scale, v_scale, what):
     """The cache in 8 bits: -> (n_pages, Hkv, page_size, dh)."""
-    _dev(k_pool, "k_pool", (torch.float8_e4m3fn,), 4), _dev(v_pool, "v_pool", (torch.float8_e4m3fn,), 4)
+    # (one expression for what holds in front of every layer's launch; where it does not, the checks below say what is wrong)
+    if (isinstance(k_pool, torch.Tensor) and k_pool.dtype is FP8 and k_pool.is_cuda and k_pool.dim() == 4 and isinstance(v_pool, torch.Tensor)
+            and v_pool.dtype is FP8 and v_pool.is_cuda and isinstance(k_scale, torch.Tensor) and isinstance(v_scale, torch.Tensor)
+            and k_scale.dtype is v_scale.dtype is torch.float32 and k_scale.is_cuda and v_scale.is_cuda):
+        n_pages, Hkv, ps, dh = shape = k_pool.shape
+        if (0 not in shape and dh <= 256 and v_pool.shape == (n_pages, Hkv, dh, ps) and k_scale.shape == v_scale.shape == (n_pages, Hkv)
+                and k_pool.is_contiguous() and v_pool.is_contiguous() and k_scale.is_contiguous() and v_scale.is_contiguous()):
+            return shape
+    _dev(k_pool, "k_pool", (FP8,), 4), _dev(v_pool, "v_pool", (FP8,), 4)
     _dev(k_scale, "k_scale", (torch.float32,), 2), _dev(v_scale, "v_scale", (torch.float32,), 2)
     n_pages, Hkv, ps, dh = k_pool.shape
     _need(k_pool.is_contiguous() and v_pool.is_contiguous() and tuple(v_pool.shape) == (n_pages, Hkv, dh, ps),
@@ -888,11 +896,21 @@ def _pools8(k_pool, v_pool, k_scale, v_scale, what):
     return n_pages, Hkv, ps, dh
 
 
-def _one_device(what, first, *others):
-    """All on one device, and that the current one: a launch goes to the current device's stream."""
-    for t in others:
-        _need(t is None or t.device == first.device, lambda: f"{what}: tensors on {first.device} and {t.device}")
-    _need(first.device.index == torch.cuda.current_device(), lambda: f"{what}: tensors on {first.device}, which is not the current device")
+FP8 = torch.float8_e4m3fn
+_device_now = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)     # (torch.cuda.current_device asks first whether CUDA is up)
+
+
+def _stream8():
+    """_stream(), for tensors that _one_device has seen on the current device."""
+    return _raw_stream(_device_now()) if _raw_stream is not None else _stream()
+
+
+def _one_device(what, *tensors):
+    """All on the current device, whose stream a launch goes to."""
+    now = _device_now()
+    for t in tensors:
+        if t is not None and t.get_device() != now:
+            raise KernelError(f"{what}: a tensor on {t.device}, the current device is {now}")
 
 
 def kv_append8(src, k_col, v_col, slot_map, k_pool, v_pool, k_scale, v_scale, positions=None, freq=None, halves=False, mag=1.0,
@@ -912,56 +930,110 @@ def kv_append8(src, k_col, v_col, slot_map, k_pool, v_pool, k_scale, v_scale, po
     freq: 32-bit [dims / 2]: the first `dims` entries of every key are turned in pairs, entries 2i and 2i + 1, or with halves i and
     i + dims / 2, by the angle positions[t] * freq[i] (cos and sin times mag; in 64 bits until the one rounding).  q_out [T, n_heads * dh] of src's
     dtype: the queries at columns q_col.. of src, turned the same way (it may be those columns themselves)."""
-    _dev(src, "src", _FLOATS, 2), _dev(slot_map, "slot_map", _I32, 1)
     n_pages, Hkv, ps, dh = _pools8(k_pool, v_pool, k_scale, v_scale, "kv_append8")
-    ld, T, w = _rows(src, "src"), src.shape[0], Hkv * dh
-    _need(slot_map.is_contiguous() and slot_map.shape[0] == T, "kv_append8: slot_map")
-    _need(0 <= k_col and k_col + w <= src.shape[1] and 0 <= v_col and v_col + w <= src.shape[1], "kv_append8: columns outside src")
+    if not _append8_holds(src, k_col, v_col, slot_map, positions, freq, q_out, q_col, n_heads, Hkv, dh):
+        _append8_checks(src, k_col, v_col, slot_map, positions, freq, q_out, q_col, n_heads, Hkv, dh)
     _one_device("kv_append8", src, slot_map, k_pool, v_pool, k_scale, v_scale, positions, freq, q_out)
-    dims = 0
+    T = src.shape[0]
+    if T == 0:
+        return
+    ld, dims = src.stride(0) if T > 1 else src.shape[1], 0 if freq is None else 2 * freq.numel()
+    ldq = 0 if q_out is None else q_out.stride(0) if T > 1 else q_out.shape[1]
+    _ok(_lib("cache8").dn_kv_append8(src.data_ptr(), ld, k_col, v_col, slot_map.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(),
+                                     k_scale.data_ptr(), v_scale.data_ptr(), n_pages, positions.data_ptr() if dims else None,
+                                     freq.data_ptr() if dims else None, dims, 1 if halves else 0, float(mag), q_col, n_heads,
+                                     q_out.data_ptr() if ldq else None, ldq, T, Hkv, dh, ps, _CODE[src.dtype], _stream8()), "kv_append8")
+
+
+def _append8_holds(src, k_col, v_col, slot_map, positions, freq, q_out, q_col, n_heads, Hkv, dh):
+    """Whether the rows of an ordinary call are right, in one expression (_append8_checks says what is wrong): queries in front of the
+    keys, and turned in memory apart from src or where they stand."""
+    if not (isinstance(src, torch.Tensor) and isinstance(slot_map, torch.Tensor) and src.is_cuda and slot_map.is_cuda and src.dim() == 2):
+        return False
+    T, width = src.shape
+    w, stride = Hkv * dh, src.stride()
+    if not (src.dtype in _CODE and stride[1] == 1 and stride[0] >= width and slot_map.dtype is torch.int32 and slot_map.shape == (T,)
+            and slot_map.is_contiguous() and 0 <= k_col <= width - w and 0 <= v_col <= width - w):
+        return False
+    if freq is None:
+        return q_out is None and n_heads == 0
+    if not (isinstance(freq, torch.Tensor) and isinstance(positions, torch.Tensor) and freq.dtype is torch.float32 and freq.is_cuda and positions.is_cuda
+            and positions.dtype is torch.int32 and positions.shape == (T,) and 2 <= 2 * freq.numel() <= dh and freq.is_contiguous()
+            and positions.is_contiguous()):
+        return False
+    if q_out is None:
+        return n_heads == 0
+    qw = n_heads * dh
+    if not (isinstance(q_out, torch.Tensor) and q_out.dtype is src.dtype and n_heads >= 1 and q_out.shape == (T, qw) and 0 <= q_col
+            and q_col + qw <= k_col <= v_col):
+        return False
+    size, at, own, sq = src.element_size(), q_out.data_ptr(), src.data_ptr(), q_out.stride()
+    return sq[1] == 1 and sq[0] >= qw and T > 1 and (at == own + q_col * size and sq[0] == stride[0] or at >= own + ((T - 1) * stride[0] + width) * size
+                                                    or at + ((T - 1) * sq[0] + qw) * size <= own)
+
+
+def _append8_checks(src, k_col, v_col, slot_map, positions, freq, q_out, q_col, n_heads, Hkv, dh):
+    _dev(src, "src", _FLOATS, 2), _dev(slot_map, "slot_map", _I32, 1)
+    ld, (T, width), w = _rows(src, "src"), src.shape, Hkv * dh
+    _need(slot_map.is_contiguous() and slot_map.shape[0] == T, "kv_append8: slot_map")
+    _need(0 <= k_col and k_col + w <= width and 0 <= v_col and v_col + w <= width, "kv_append8: columns outside src")
     if freq is not None:
         _f32vec(freq, "freq")
-        dims = 2 * freq.numel()
-        _need(2 <= dims <= dh, lambda: f"kv_append8: {freq.numel()} frequencies for heads of {dh}")
+        _need(2 <= 2 * freq.numel() <= dh, lambda: f"kv_append8: {freq.numel()} frequencies for heads of {dh}")
         _need(positions is not None, "kv_append8: a turn needs positions")
         _dev(positions, "positions", _I32, 1)
         _need(positions.is_contiguous() and positions.shape[0] == T, "kv_append8: positions")
-    ldq = 0
-    if q_out is not None:
-        _need(dims > 0, "kv_append8: queries are only turned here; without a turn they are src's own columns")
-        _dev(q_out, "q_out", (src.dtype,), 2)
-        qw = n_heads * dh
-        _need(n_heads >= 1 and tuple(q_out.shape) == (T, qw) and 0 <= q_col and q_col + qw <= src.shape[1], "kv_append8: queries")
-        _need(q_col + qw <= min(k_col, v_col) or q_col >= max(k_col, v_col) + w or (k_col + w <= q_col and q_col + qw <= v_col)
-              or (v_col + w <= q_col and q_col + qw <= k_col), "kv_append8: the queries' columns are keys' or values' too")
-        ldq = _rows(q_out, "q_out")
-        size = src.element_size()
-        there, first, own_first = q_out.data_ptr() == src.data_ptr() + q_col * size and (ldq == ld or T == 1), q_out.data_ptr(), src.data_ptr()
-        _need(there or T == 0 or first >= own_first + ((T - 1) * ld + src.shape[1]) * size or first + ((T - 1) * ldq + qw) * size <= own_first,
-              "kv_append8: q_out is either src's own query columns or memory apart from src")
-    else:
+    if q_out is None:
         _need(n_heads == 0, "kv_append8: n_heads goes with q_out")
-    if T == 0:
         return
-    _ok(_lib("cache8").dn_kv_append8(src.data_ptr(), ld, k_col, v_col, slot_map.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(),
-                                     k_scale.data_ptr(), v_scale.data_ptr(), n_pages, _ptr(positions if dims else None), _ptr(freq), dims,
-                                     int(bool(halves)), float(mag), q_col, n_heads, _ptr(q_out), ldq, T, Hkv, dh, ps, _CODE[src.dtype],
-                                     _stream()), "kv_append8")
+    _need(freq is not None, "kv_append8: queries are only turned here; without a turn they are src's own columns")
+    _dev(q_out, "q_out", (src.dtype,), 2)
+    qw = n_heads * dh
+    _need(n_heads >= 1 and tuple(q_out.shape) == (T, qw) and 0 <= q_col and q_col + qw <= width, "kv_append8: queries")
+    _need(q_col + qw <= min(k_col, v_col) or q_col >= max(k_col, v_col) + w or (k_col + w <= q_col and q_col + qw <= v_col)
+          or (v_col + w <= q_col and q_col + qw <= k_col), "kv_append8: the queries' columns are keys' or values' too")
+    ldq = _rows(q_out, "q_out")
+    size, first, own_first = src.element_size(), q_out.data_ptr(), src.data_ptr()
+    there = first == own_first + q_col * size and (ldq == ld or T == 1)
+    _need(there or T == 0 or first >= own_first + ((T - 1) * ld + width) * size or first + ((T - 1) * ldq + qw) * size <= own_first,
+          "kv_append8: q_out is either src's own query columns or memory apart from src")
 
 
 def _single8_shape(n_tiles, n_heads, Hkv, dh, max_context, window, keep_first):
-    """-> (waves of a workgroup, workgroups that a row's keys are shared out to)."""
+    """-> (waves of a workgroup, workgroups that a row's keys are shared out to).  One workgroup per CU, as long as every wave has two tiles of
+    64 keys: a row over 131,072 keys with 8 key heads of 128 takes 58 us in 32 x 8 workgroups, 62 in 16 x 8 and 75 in 64 x 8; 518 keys with 25
+    heads of 64 5.0 us undivided and 7.0 in two.  Workgroups of 8 waves (two of them, or heads beyond 128, fill the registers): 16 rows in a window
+    of 4,096 26.8 us, in 4 waves 29.5; 64 rows of GPT-2 XL 24.6 and 25.3."""
     reach = max_context if window == 0 else min(max_context, window + keep_first + 128)
-    tiles = -(-reach // 64)
     groups = n_tiles * Hkv * -(-(n_heads // Hkv) // 16)
-    waves = 8 if dh <= 128 and groups < 1024 and tiles > 4 else 4
-    n_splits = max(1, min(-(-tiles // waves), 1024 // groups))
-    return waves, n_splits
+    waves = 8 if dh <= 128 else 4
+    return waves, max(1, min(-(-reach // 64) // (2 * waves), 256 // groups))
 
 
 def _portions8_shape(n_tiles, n_heads, dh):
     """-> (groups of 32 rows, groups of keys) of a workgroup of the portions' kernel."""
     return 4, 1
+
+
+def _attention8_holds(q, out, block_tables, tiles, n_heads, Hkv, dh):
+    """Whether the rows and tables of an ordinary call are right, in one expression (_attention8_checks says what is wrong)."""
+    if not (isinstance(q, torch.Tensor) and isinstance(out, torch.Tensor) and isinstance(block_tables, torch.Tensor) and isinstance(tiles, torch.Tensor)
+            and q.is_cuda and out.is_cuda and block_tables.is_cuda and tiles.is_cuda and q.dim() == 2 and out.dim() == 2 and n_heads > 0):
+        return False
+    T, width = q.shape
+    w, sq, so = n_heads * dh, q.stride(), out.stride()
+    return (q.dtype in _CODE and out.dtype is q.dtype and block_tables.dtype is tiles.dtype is torch.int32 and n_heads % Hkv == 0 and width >= w
+            and out.shape == (T, w) and sq[1] == so[1] == 1 and sq[0] >= width and so[0] >= w and block_tables.dim() == 2 and tiles.dim() == 2
+            and tiles.shape[0] == 4 and block_tables.is_contiguous() and tiles.is_contiguous())
+
+
+def _attention8_checks(q, out, block_tables, tiles, n_heads, Hkv, dh):
+    _dev(q, "q", _FLOATS, 2), _dev(out, "out", (q.dtype,), 2)
+    _dev(block_tables, "block_tables", _I32, 2), _dev(tiles, "tiles", _I32, 2)
+    _need(n_heads >= 1 and n_heads % Hkv == 0, lambda: f"attention8: {n_heads} heads over {Hkv} key heads")
+    _need(q.shape[1] >= n_heads * dh and tuple(out.shape) == (q.shape[0], n_heads * dh), "attention8: q/out shapes")
+    _need(block_tables.is_contiguous() and tiles.is_contiguous() and tiles.shape[0] == 4, "attention8: tables")
+    _rows(q, "q"), _rows(out, "out")
 
 
 def attention8(q, out, k_pool, v_pool, k_scale, v_scale, block_tables, tiles, n_heads, scale, window=0, tiles_wide=None,
@@ -978,20 +1050,18 @@ def attention8(q, out, k_pool, v_pool, k_scale, v_scale, block_tables, tiles, n_
     becomes softcap * tanh(s / softcap).
     Rows of padding tiles are left as they were.  What stands in places that a row does not read does not reach it, NaN included;
     a page that is given back (a negative entry) is not read; a row that reads nothing becomes zeros."""
-    _dev(q, "q", _FLOATS, 2), _dev(out, "out", (q.dtype,), 2)
     n_pages, Hkv, ps, dh = _pools8(k_pool, v_pool, k_scale, v_scale, "attention8")
-    _dev(block_tables, "block_tables", _I32, 2), _dev(tiles, "tiles", _I32, 2)
-    T = q.shape[0]
-    _need(n_heads >= 1 and n_heads % Hkv == 0, lambda: f"attention8: {n_heads} heads over {Hkv} key heads")
-    _need(q.shape[1] >= n_heads * dh and tuple(out.shape) == (T, n_heads * dh), "attention8: q/out shapes")
-    _need(block_tables.is_contiguous() and tiles.is_contiguous() and tiles.shape[0] == 4, "attention8: tables")
-    ldq, ldo = _rows(q, "q"), _rows(out, "out")
     sink_at, sink = (sink, True) if isinstance(sink, torch.Tensor) else (None, bool(sink))
-    _f32vec(sink_at, "sink", n_heads)
-    _need(window >= 0 and softcap >= 0, "attention8: window or softcap")
     keep_first = int(keep_first) if window > 0 else 0      # (without a window every key is read anyway)
+    if not _attention8_holds(q, out, block_tables, tiles, n_heads, Hkv, dh):
+        _attention8_checks(q, out, block_tables, tiles, n_heads, Hkv, dh)
+    if sink_at is not None:
+        _f32vec(sink_at, "sink", n_heads)
+    _need(window >= 0 and softcap >= 0, "attention8: window or softcap")
     _need(keep_first >= 0, "attention8: keep_first")
     _one_device("attention8", q, out, k_pool, v_pool, k_scale, v_scale, block_tables, tiles, tiles_wide, sink_at)
+    T = q.shape[0]
+    ldq, ldo = (q.stride(0), out.stride(0)) if T > 1 else (q.shape[1], out.shape[1])
     n_tiles = tiles.shape[1]
     if T == 0 or n_tiles == 0:
         return out
@@ -1007,7 +1077,7 @@ def attention8(q, out, k_pool, v_pool, k_scale, v_scale, block_tables, tiles, n_
                 q.data_ptr(), ldq, out.data_ptr(), ldo, k_pool.data_ptr(), v_pool.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
                 n_pages, block_tables.data_ptr(), block_tables.shape[1], base, base + 4 * n_tiles, base + 12 * n_tiles, n_tiles, _ptr(part),
                 n_splits, waves, n_heads, Hkv, dh, ps, float(scale), int(window), keep_first, int(sink), _ptr(sink_at), float(softcap),
-                _CODE[q.dtype], _stream()), "attention8 (single rows)")
+                _CODE[q.dtype], _stream8()), "attention8 (single rows)")
             return out
     # (the portions' kernel takes the largest score for the largest product: a scale that is not positive goes the plain way)
     if aligned and tiles_wide is not None and scale > 0 and ldq % 8 == 0 and q.data_ptr() % 16 == 0:
@@ -1020,12 +1090,12 @@ def attention8(q, out, k_pool, v_pool, k_scale, v_scale, block_tables, tiles, n_
             q.data_ptr(), ldq, out.data_ptr(), ldo, k_pool.data_ptr(), v_pool.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
             n_pages, block_tables.data_ptr(), block_tables.shape[1], base, base + 4 * n_wide, base + 8 * n_wide, base + 12 * n_wide, n_wide,
             rows, groups, n_heads, Hkv, dh, ps, float(scale), int(window), keep_first, int(sink), _ptr(sink_at), float(softcap),
-            _CODE[q.dtype], _stream()), "attention8 (portions)")
+            _CODE[q.dtype], _stream8()), "attention8 (portions)")
         return out
     _ok(_lib("cache8").dn_attention8(
         q.data_ptr(), ldq, out.data_ptr(), ldo, k_pool.data_ptr(), v_pool.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), n_pages,
         block_tables.data_ptr(), block_tables.shape[1], base, base + 4 * n_tiles, base + 8 * n_tiles, base + 12 * n_tiles, n_tiles, n_heads,
-        Hkv, dh, ps, float(scale), int(window), keep_first, int(sink), _ptr(sink_at), float(softcap), _CODE[q.dtype], _stream()), "attention8")
+        Hkv, dh, ps, float(scale), int(window), keep_first, int(sink), _ptr(sink_at), float(softcap), _CODE[q.dtype], _stream8()), "attention8")
     return out
 
 
