@@ -88,6 +88,7 @@ class Workloads:
         live = max(64, a.batch)
         self.opts = EngineOptions(dtype=dtype, page_size=a.page_size, cache_tokens=live * P, max_live=live, max_batch_tokens=4096,
                                   prefill_chunk=1024, use_graphs=not (a.no_graphs or a.kernel_times), seed=0,
+                                  cache_dtype=getattr(a, "cache_dtype", None),
                                   norms_inside_products=not a.norm_kernels, deferred_sums=not a.no_deferred_sums)
         self.runner = ModelRunner.from_random(self.cfg, seed=0, options=self.opts, stored=dtype)
         self.gen = torch.Generator().manual_seed(0)
@@ -188,6 +189,7 @@ def main():
     ap.add_argument("--batch", type=int, default=8)
     ap.add_argument("--context", type=int, default=512)
     ap.add_argument("--dtype", default="bfloat16", choices=["bfloat16", "float32"])
+    ap.add_argument("--cache-dtype", default=None, choices=["float8"], help="--only decode, prefill: keys and values in 8 bits")
     ap.add_argument("--layers", type=int, default=0, help="fewer layers than the configuration (0: all)")
     ap.add_argument("--no-graphs", action="store_true")
     ap.add_argument("--norm-kernels", action="store_true",
@@ -214,6 +216,8 @@ def main():
                          "BASELINE.json's configs[3], GPT-2 Large shape, 64 requests through the scheduler; replay: "
                          "configs[4], GPT-2 Medium shape, against the plain implementation)")
     a = ap.parse_args()
+    if a.only not in ("decode", "prefill") and a.cache_dtype:
+        ap.error("--cache-dtype goes with --only decode or --only prefill")
     if a.gpus != 1:
         print(f"bench.py: this engine runs on one GPU; --gpus {a.gpus} is not supported")
         sys.exit(2)

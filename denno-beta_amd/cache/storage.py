@@ -4,7 +4,8 @@ Each cache that the model's run order names has a need (PagedKV or FixedState, f
 mixer).  Caches with the same need form a group: a paged group has one pool of pages,
 [caches, n_pages, Hkv, page_size, dh] for keys and [caches, n_pages, Hkv, dv, page_size] for
 values (a page's values transposed, as attention's second product reads them; dv is dh unless
-the need names a width of its own for values), and one block table per request, shared by the group's caches; a state group has [caches, slots, *shape] and is
+the need names a width of its own for values; in 8 bits (kv_dtype torch.float8_e4m3fn) beside them a 32-bit scale per page and head for keys, and one for values,
+[caches, n_pages, Hkv]), and one block table per request, shared by the group's caches; a state group has [caches, slots, *shape] and is
 indexed by the request's slot.  Groups with different needs (all keys, a window of them)
 draw from pools of their own.
 """
@@ -51,13 +52,16 @@ class CacheStorage:
                 raise TypeError(f"unknown cache need {cs!r}")
         self.layouts = layouts
         self.manager = CacheManager(layouts, max_live)
-        self.k, self.v, self.state = [], [], []
+        self.k, self.v, self.state, self.k_scale, self.v_scale = [], [], [], [], []
         for g, cs in enumerate(self.group_specs):
             n = len(self.members[g])
+            scales = isinstance(cs, PagedKV) and allocate and self._dtype(cs) == torch.float8_e4m3fn
+            for into in (self.k_scale, self.v_scale):
+                into.append(torch.zeros((n, n_pages, cs.n_kv_heads), dtype=torch.float32, device=device) if scales else None)
             if isinstance(cs, PagedKV):
                 shape = (n, n_pages, cs.n_kv_heads, page_size, cs.head_dim)
                 vshape = (n, n_pages, cs.n_kv_heads, cs.v_dim, page_size)   # a page's values transposed
-                dt = _TORCH[cs.dtype] if cs.dtype is not None else kv_dtype
+                dt = self._dtype(cs)
                 if allocate:
                     # zeros, not empty: a page's unwritten tail is read (masked) by attention,
                     # and must hold numbers, not whatever bits the allocator left
@@ -71,6 +75,9 @@ class CacheStorage:
                 self.state.append(torch.zeros((n, max_live) + tuple(cs.shape), dtype=_TORCH[cs.dtype],
                                               device=device) if allocate else None)
 
+    def _dtype(self, cs: PagedKV) -> torch.dtype:
+        return _TORCH[cs.dtype] if cs.dtype is not None else self.kv_dtype
+
     @property
     def n_groups(self):
         return len(self.group_specs)
@@ -83,6 +90,8 @@ class CacheStorage:
         if g < 0:
             return CacheView(group=-1, writes=writes)
         if isinstance(self.group_specs[g], PagedKV):
+            if self.k_scale[g] is not None:
+                return CacheView(group=g, writes=writes, k=self.k[g][j], v=self.v[g][j], k_scale=self.k_scale[g][j], v_scale=self.v_scale[g][j])
             return CacheView(group=g, writes=writes, k=self.k[g][j], v=self.v[g][j])
         return CacheView(group=g, writes=writes, state=self.state[g][j])
 
@@ -103,6 +112,8 @@ class CacheStorage:
         total = 0
         for g, cs in enumerate(self.group_specs):
             if isinstance(cs, PagedKV):
-                dt = _TORCH[cs.dtype] if cs.dtype is not None else self.kv_dtype
+                dt = self._dtype(cs)
                 total += len(self.members[g]) * cs.n_kv_heads * (cs.head_dim + cs.v_dim) * torch.empty((), dtype=dt).element_size()
+                if dt == torch.float8_e4m3fn:       # (a page's two scales, shared out to its tokens)
+                    total += -(-len(self.members[g]) * cs.n_kv_heads * 8 // self.page_size)
         return total

@@ -18,7 +18,7 @@ for token ids where the folder has no tokenizer.json, `--top-k`, `--top-p`, `--s
 request parameters, crates/denno-engine/src/engine.rs:42-44), `--ignore-eos`; `--prompt-file` with
 one prompt a line (token ids separated by commas or blanks), which all go through the scheduler
 together, one line of output each in the file's order; and the engine's own options (`--max-live`,
-`--page-size`, `--cache-tokens`, `--prefill-chunk`, `--max-batch-tokens`, `--kv-policy`,
+`--page-size`, `--cache-tokens`, `--cache-dtype`, `--prefill-chunk`, `--max-batch-tokens`, `--kv-policy`,
 `--no-graphs`), which the reference sets through DENNO_* environment variables.
 """
 from __future__ import annotations
@@ -80,6 +80,8 @@ def parser():
     g.add_argument("--page-size", type=int, default=16, help="tokens in a page of the cache")
     g.add_argument("--cache-tokens", type=int, default=None,
                    help="size of the cache in tokens (default: max-live times the model's positions)")
+    g.add_argument("--cache-dtype", default=None, choices=["float8"],
+                   help="keep keys and values in 8 bits, with a scale per page and head (default: the precision that --quant names)")
     g.add_argument("--prefill-chunk", type=int, default=512, help="longest portion of one prompt in one step")
     g.add_argument("--max-batch-tokens", type=int, default=2048, help="token budget of one step")
     g.add_argument("--kv-policy", default="preempt", choices=["preempt", "reserve"],
@@ -128,7 +130,7 @@ def cmd_generate(a):
         raise SystemExit(f"--stop is a text: {a.model} has no tokenizer.json (or the tokenizers package is missing)")
     max_live = a.max_live if a.max_live is not None else min(len(prompts), 64)
     eng = Engine.from_folder(a.model, EngineOptions(
-        dtype=quant, max_live=max_live, seed=a.seed, page_size=a.page_size, cache_tokens=a.cache_tokens,
+        dtype=quant, max_live=max_live, seed=a.seed, page_size=a.page_size, cache_tokens=a.cache_tokens, cache_dtype=a.cache_dtype,
         prefill_chunk=a.prefill_chunk, max_batch_tokens=a.max_batch_tokens, kv_policy=a.kv_policy,
         use_graphs=not a.no_graphs), a.cast_weights,
         detokenize=(lambda ids: tok.decode(list(ids))) if tok is not None else None)

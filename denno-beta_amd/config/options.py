@@ -11,6 +11,7 @@ from typing import Optional
 
 DTYPES = ("bfloat16", "float32")
 KV_POLICIES = ("preempt", "reserve")
+CACHE_DTYPES = (None, "float8")
 
 
 @dataclass
@@ -29,10 +30,13 @@ class EngineOptions:
     seed: Optional[int] = None         # default seed of requests that bring none
     deferred_sums: bool = True         # steps of 65 to 512 rows: a product into the stream with few columns leaves its sum for the next norm's kernel (parts/blocks.py)
     norms_inside_products: bool = True  # steps of few rows: a norm between two products runs inside them (parts/blocks.py)
+    cache_dtype: Optional[str] = None  # "float8": keys and values in 8 bits (e4m3 numbers, a scale per page and head); None: dtype's
 
     def validate(self):
         if self.dtype not in DTYPES:
             raise ValueError(f"dtype must be one of {DTYPES}, got {self.dtype!r}")
+        if self.cache_dtype not in CACHE_DTYPES:
+            raise ValueError(f"cache_dtype must be one of {CACHE_DTYPES}, got {self.cache_dtype!r}")
         if self.kv_policy not in KV_POLICIES:
             raise ValueError(f"kv_policy must be one of {KV_POLICIES}, got {self.kv_policy!r}")
         if self.page_size < 1:

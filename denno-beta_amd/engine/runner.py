@@ -19,6 +19,16 @@ from .batch import StepEntry, build_context
 from .graphs import DecodeGraphs, wanted_rows
 
 _ACT = {"bfloat16": torch.bfloat16, "float32": torch.float32}
+_CACHE = {None: None, "float8": torch.float8_e4m3fn}      # None: the activations' dtype
+
+
+def refuse_8_bits(model):
+    """ValueError, naming the kinds, if a mixer that keeps pages of the engine's dtype does not keep them in 8 bits."""
+    from ..parts.base import PagedKV
+    kinds = {getattr(m, "kind_name", type(m).__name__) for b in model.blocks for m in b.mixers()
+             if isinstance(m.cache_spec(), PagedKV) and m.cache_spec().dtype is None and not m.keeps_8_bits}
+    if kinds:
+        raise ValueError(f"cache_dtype: this model's {', '.join(sorted(kinds))} keeps no cache in 8 bits")
 
 
 class ModelRunner:
@@ -30,6 +40,8 @@ class ModelRunner:
                                norms_inside_products=options.norms_inside_products,
                                deferred_sums=options.deferred_sums)
         model = spec.instantiate()
+        if options.cache_dtype is not None:
+            refuse_8_bits(model)
         if self.device.type == "cuda":
             # what this model needs is compiled now, side by side, if it is not built yet (else each library
             # would be compiled at its first call, one after the other)
@@ -37,10 +49,11 @@ class ModelRunner:
             from ..parts.base import PagedKV
             paged = any(isinstance(cs, PagedKV) for cs in model.cache_specs)
             more = sorted({lib for p in model.all_parts() for lib in getattr(p, "libraries", ())})
-            ensure_built(["host", "elementwise", "gemm"] + (["attention"] if paged else []) + more)
+            cache8 = ["cache8"] if paged and options.cache_dtype == "float8" else []
+            ensure_built(["host", "elementwise", "gemm"] + (["attention"] if paged else []) + cache8 + more)
         self.model = model.bind(tensors, self.runtime)
         cache_tokens = options.cache_tokens or options.max_live * spec.max_positions
-        self.cache = CacheStorage(self.model.cache_specs, kv_dtype=self.runtime.act_dtype,
+        self.cache = CacheStorage(self.model.cache_specs, kv_dtype=_CACHE[options.cache_dtype] or self.runtime.act_dtype,
                                   page_size=options.page_size, cache_tokens=cache_tokens,
                                   max_live=options.max_live, device=self.device)
         self.notes: List[str] = []

@@ -106,6 +106,9 @@ class Part:
     captured once as a HIP graph and replayed over new tables."""
     graph_safe = False
     libraries = ()     # kernel libraries (names in build.LIBRARIES) beyond the ones every model needs
+    # a mixer that writes and reads pages in 8 bits where the engine keeps them so (EngineOptions.cache_dtype): its CacheView then
+    # has k_scale and v_scale, and it calls ops.kv_append8 and ops.attention8
+    keeps_8_bits = False
 
     def param_specs(self) -> List[ParamSpec]:
         return []

@@ -116,6 +116,10 @@ class CausalSelfAttention(Part):
     def cache_spec(self):
         return PagedKV(self.n_kv_heads, self.kept_dim, self.window, keep_first=self.keep_first)
 
+    @property
+    def keeps_8_bits(self):
+        return not (self.split or self.prepared)
+
     def bind(self, tensors, runtime):
         super().bind(tensors, runtime)
         self.qkv.bind(tensors)
@@ -215,10 +219,34 @@ class CausalSelfAttention(Part):
             return self.out(o, out_dtype=torch.float32)
         self.out(o, residual=accumulate_into)
 
+    def _attend_8_bits(self, h, ctx, cache, g, position):
+        """The projection's rows, keys and values from there to pages in 8 bits (queries and keys turned on the way, where the
+        position encoding has a table of frequencies for whole heads), and the attention over those."""
+        act = self.runtime.act_dtype
+        qkv = self.qkv(h, out_dtype=act)
+        q, kv = qkv[:, :self.q_width], qkv[:, self.q_width:self.q_width + self.kv_width]
+        turns = position is not None and getattr(position, "rotates", False)
+        here = turns and cache.writes and hasattr(position, "freq") and getattr(position, "head_dim", 0) == self.head_dim and position.dims > 0
+        if turns and not here:
+            position.rotate(q, kv, ctx)
+        if cache.writes:
+            turn = dict(positions=ctx.positions, freq=position.freq, halves=getattr(position, "halves", False), mag=position.mag, q_out=q,
+                        q_col=0, n_heads=self.n_heads) if here else {}
+            ops.kv_append8(qkv, self.q_width, self.q_width + self.kv_width, g.slot_map, cache.k, cache.v, cache.k_scale, cache.v_scale, **turn)
+        return ops.attention8(q, torch.empty((h.shape[0], self.q_width), dtype=act, device=h.device), cache.k, cache.v, cache.k_scale,
+                              cache.v_scale, g.block_tables, g.tiles, self.n_heads, self.scale, self.window, tiles_wide=g.tiles_wide,
+                              single_rows=g.single_rows, max_context=g.max_context, sink=self.sink, keep_first=self.keep_first,
+                              softcap=self.softcap)
+
     def forward(self, h, ctx, cache, accumulate_into, stats=None, deferred=None):
         act = self.runtime.act_dtype
         g = ctx.groups[cache.group]
         position = self.position if self.position is not None else self.runtime.position
+        if cache.k_scale is not None:
+            o = self._attend_8_bits(h, ctx, cache, g, position)
+            if accumulate_into is None:
+                return self.out(o, out_dtype=torch.float32)
+            return self.out(o, residual=accumulate_into, stats=stats, deferred=deferred)
         if self.prepared:
             return self._forward_prepared(h, ctx, cache, g, position, accumulate_into)
         if self.split:

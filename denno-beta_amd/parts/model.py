@@ -104,6 +104,8 @@ class CacheView:
     k: Optional[torch.Tensor] = None       # paged: [n_pages, Hkv, page_size, dh] of this call's cache
     v: Optional[torch.Tensor] = None       #        [n_pages, Hkv, dh, page_size]
     state: Optional[torch.Tensor] = None   # fixed state: [n_slots, *shape]
+    k_scale: Optional[torch.Tensor] = None   # pages in 8 bits: 32-bit [n_pages, Hkv], what a number of k is multiplied with; None: k and v as they are
+    v_scale: Optional[torch.Tensor] = None
 
 
 class DecoderModel:
