@@ -22,7 +22,7 @@ struct Args {
   const float *k_scale, *v_scale;
   const int32_t *block_tables, *tile_seq, *tile_row0, *tile_nrows, *tile_pos0;
   const float* sink_at;
-  int ldq, ldo, n_pages, max_blocks, H, Hkv, page_size, window, keep, sink;
+  int ldq, ldo, n_pages, max_blocks, H, Hkv, page_shift, window, keep, sink;      // pages of 1 << page_shift keys
   float scale, cap;
 };
 
@@ -38,7 +38,7 @@ __device__ __forceinline__ u32x4 widen_scaled(uint32_t lo, uint32_t hi, float sc
 // A wait for products that are read behind a branch, which the compiler does not always leave room for: 16 cycles, as a product of 32 x 32 wants at least
 __device__ __forceinline__ void settle(floatx16& a, floatx16& b) { asm volatile("s_nop 15" : "+v"(a), "+v"(b)); }
 
-// whether one of a word's four e4m3 numbers is NaN (0x7f or 0xff)
+// the upper bit of those of a word's four e4m3 numbers that are NaN (0x7f or 0xff)
 __device__ __forceinline__ uint32_t nan_in(uint32_t w) { return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
 
 template <int DH16, int PARTS, int RG, int KG>
@@ -60,7 +60,8 @@ __global__ __launch_bounds__(64 * RG * KG) __attribute__((amdgpu_waves_per_eu(wa
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
   bf16_t* const tiles = reinterpret_cast<bf16_t*>(smem);                        // [2][KG][keys | values]
   constexpr int FLAGS_AT = BYTES_TILES > BYTES_JOIN ? BYTES_TILES : BYTES_JOIN;
-  int* const flags = reinterpret_cast<int*>(smem + FLAGS_AT);                   // [2][KG][4 blocks: whether there is a page | RG waves: NaN among values]
+  int* const flags = reinterpret_cast<int*>(smem + FLAGS_AT);                   // [2][KG][4 blocks: whether there is a page]
+  int* const seen = flags + 2 * KG * 4;                                         // whether there was a value that is NaN
 
   // consecutive workgroups go to different XCDs: the heads of one key head are Hkv workgroups apart, so that with 8 key heads (or a
   // multiple) an XCD's L2 holds the keys of its own heads only
@@ -75,7 +76,6 @@ __global__ __launch_bounds__(64 * RG * KG) __attribute__((amdgpu_waves_per_eu(wa
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64;
   const int kg = wave / RG, rg = wave % RG, t = threadIdx.x % THREADS;
   const int col = lane % 32, g = lane / 32;
-  const int ps = a.page_size;
   const int32_t* bt = a.block_tables + static_cast<size_t>(seq) * a.max_blocks;
   const int wrow0 = rg * 32;
   const bool has_rows = wrow0 < nrows;      // (a wave without rows carries tiles all the same)
@@ -115,71 +115,80 @@ __global__ __launch_bounds__(64 * RG * KG) __attribute__((amdgpu_waves_per_eu(wa
   auto key_of = [&](int i) { return STEP * (i < kept ? i : rest + i - kept); };
 
   // This thread's chunks of its group's tile: chunk x = t + THREADS u is, of the keys, 16 dims (x % DH16) of key x / DH16; of the
-  // values, the 16 keys of block x % 4 of dim x / 4 (the same block for every u).
-  auto page_of = [&](int key) {      // of the block of 16 that begins with key; -1: none, or behind the last row
-    const int b = key / ps;
-    const int page = key <= hi_g && b < a.max_blocks ? bt[b] : -1;
-    return page < a.n_pages ? page : -1;
-  };
-  int k_page[U], v_page;
+  // values, the 16 keys of block x % 4 of dim x / 4 (the same block for every u).  A tile begins at a multiple of 64, so in pages of up to
+  // 64 keys a chunk's place in its page is always the same, and in longer ones what is added to it is the same for all threads.
+  const int in_page = (1 << a.page_shift) - 1;
+  const uint32_t page_bytes = static_cast<uint32_t>(a.Hkv) * DH << a.page_shift;
+  int k_key[U], k_page[U], v_page;
+  uint32_t k_at[U], v_at[U];
   u32x4 k_raw[U], v_raw[U];
   float k_by[U], v_by;
-  int k_key[U];
+  bool v_there = false;      // whether the values in registers have a page
+  const int v_block = 16 * (t % 4);
 #pragma unroll
-  for (int u = 0; u < U; ++u) k_key[u] = min(t + THREADS * u, CHUNKS - 1) / DH16;
-  auto pages = [&](int i) {
-    const int kt = key_of(i) + 64 * kg;
-#pragma unroll
-    for (int u = 0; u < U; ++u) k_page[u] = i < steps ? page_of(kt + (k_key[u] & ~15)) : -1;
-    v_page = i < steps ? page_of(kt + 16 * (t % 4)) : -1;
+  for (int u = 0; u < U; ++u) {
+    const int x = min(t + THREADS * u, CHUNKS - 1);
+    k_key[u] = x / DH16;
+    k_at[u] = ((hk << a.page_shift) + (k_key[u] & in_page)) * DH + x % DH16 * 16;
+    v_at[u] = ((hk * DH + x / 4) << a.page_shift) + (v_block & in_page);
+  }
+  // the page of the block of 16 keys that key kt + off stands in (off < 64); -1: none, or behind the last row
+  auto page_of = [&](int kt, int off) {
+    const int b = (kt >> a.page_shift) + (off >> a.page_shift);
+    const int page = bt[min(b, a.max_blocks - 1)];
+    return b < a.max_blocks && kt + (off & ~15) <= hi_g && page < a.n_pages ? page : -1;
   };
-  int v_there = 0;      // whether the values in registers have a page
-  auto fetch = [&](int i) {      // (what has no page reads the pools' first and is stored as zeros)
-    const int kt = key_of(i) + 64 * kg;
+  auto pages = [&](int i) {
+    const int kt = key_of(i) + 64 * kg;      // (a step behind the last one begins behind the last row)
+#pragma unroll
+    for (int u = 0; u < U; ++u) k_page[u] = page_of(kt, k_key[u]);
+    v_page = page_of(kt, v_block);
+  };
+  auto fetch = [&](int i) {      // (what has no page reads the pools' first: no row reads what comes of it)
+    const int kt = key_of(i) + 64 * kg, far = kt & in_page;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const size_t ph = static_cast<size_t>(max(k_page[u], 0)) * a.Hkv + hk;
-      k_raw[u] = *reinterpret_cast<const u32x4*>(a.k_pool + (ph * ps + (kt + k_key[u]) % ps) * DH + min(t + THREADS * u, CHUNKS - 1) % DH16 * 16);
-      k_by[u] = a.k_scale[ph];
-      if (k_page[u] < 0) k_by[u] = -1.f;      // (settled when the chunk is stored)
+      const uint32_t page = max(k_page[u], 0);
+      k_raw[u] = *reinterpret_cast<const u32x4*>(a.k_pool + static_cast<size_t>(page) * page_bytes + (k_at[u] + far * DH));
+      k_by[u] = a.k_scale[page * a.Hkv + hk];
     }
-    const size_t ph = static_cast<size_t>(max(v_page, 0)) * a.Hkv + hk;
-    v_by = a.v_scale[ph];
+    const uint32_t page = max(v_page, 0);
+    v_by = a.v_scale[page * a.Hkv + hk];
     v_there = v_page >= 0;
 #pragma unroll
-    for (int u = 0; u < U; ++u)
-      v_raw[u] = *reinterpret_cast<const u32x4*>(a.v_pool + (ph * DH + min(t + THREADS * u, CHUNKS - 1) / 4) * ps + (kt + 16 * (t % 4)) % ps);
+    for (int u = 0; u < U; ++u) v_raw[u] = *reinterpret_cast<const u32x4*>(a.v_pool + static_cast<size_t>(page) * page_bytes + (v_at[u] + far));
   };
-  const u32x4 zero4 = {0u, 0u, 0u, 0u};
   auto stash = [&](int i, int buf) {
     bf16_t* dst = tiles + (buf * KG + kg) * TSZ;
-    int* flag = flags + (buf * KG + kg) * (4 + RG);
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int x = t + THREADS * u;
-      if (CHUNKS % THREADS == 0 || x < CHUNKS) {
-        const bool ok = k_by[u] >= 0.f;
-        u32x4* to = reinterpret_cast<u32x4*>(dst + x / DH16 * KROW + x % DH16 * 16);
-        to[0] = ok ? widen_scaled(k_raw[u][0], k_raw[u][1], k_by[u]) : zero4;
-        to[1] = ok ? widen_scaled(k_raw[u][2], k_raw[u][3], k_by[u]) : zero4;
-      }
-    }
+    // Values that are NaN go in as zeros (a weight of zero, of a row that does not read the value, would make NaN of its result), and the
+    // rows that do read them are seen to at the end.
     uint32_t nan = 0;
 #pragma unroll
+    for (int u = 0; u < U; ++u) nan |= nan_in(v_raw[u][0]) | nan_in(v_raw[u][1]) | nan_in(v_raw[u][2]) | nan_in(v_raw[u][3]);
+    if (__builtin_amdgcn_ballot_w64(nan != 0) != 0) {
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int w = 0; w < 4; ++w) v_raw[u][w] &= ~((nan_in(v_raw[u][w]) >> 7) * 0xffu);
+      if (nan != 0 && v_there) *seen = 1;
+    }
+#pragma unroll
     for (int u = 0; u < U; ++u) {
       const int x = t + THREADS * u;
       if (CHUNKS % THREADS == 0 || x < CHUNKS) {
-        u32x4* to = reinterpret_cast<u32x4*>(dst + KSZ + x / 4 * VROW + x % 4 * 16);
-        to[0] = v_there ? widen_scaled(v_raw[u][0], v_raw[u][2], v_by) : zero4;
-        to[1] = v_there ? widen_scaled(v_raw[u][1], v_raw[u][3], v_by) : zero4;
-        nan |= nan_in(v_raw[u][0]) | nan_in(v_raw[u][1]) | nan_in(v_raw[u][2]) | nan_in(v_raw[u][3]);
+        u32x4* to = reinterpret_cast<u32x4*>(dst + x / DH16 * KROW + x % DH16 * 16);
+        to[0] = widen_scaled(k_raw[u][0], k_raw[u][1], k_by[u]);
+        to[1] = widen_scaled(k_raw[u][2], k_raw[u][3], k_by[u]);
+        to = reinterpret_cast<u32x4*>(dst + KSZ + x / 4 * VROW + x % 4 * 16);
+        to[0] = widen_scaled(v_raw[u][0], v_raw[u][2], v_by);
+        to[1] = widen_scaled(v_raw[u][1], v_raw[u][3], v_by);
       }
     }
-    if (t < 4) flag[t] = v_there;
-    const uint64_t any = __builtin_amdgcn_ballot_w64((nan != 0) & (v_there != 0));
-    if (lane == 0) flag[4 + rg] = any != 0;
+    if (t < 4) flags[(buf * KG + kg) * 4 + t] = v_there;
   };
 
+  if (threadIdx.x == 0) *seen = 0;
+  __syncthreads();
   pages(0);
   fetch(0);
   pages(1);
@@ -198,7 +207,7 @@ __global__ __launch_bounds__(64 * RG * KG) __attribute__((amdgpu_waves_per_eu(wa
     if (has_rows && kw <= hi_w && (kw + 63 >= lo_w || kw < a.keep)) {
       const bf16_t* Kb = tiles + (buf * KG + kg) * TSZ;
       const bf16_t* Vb = Kb + KSZ;
-      const int* flag = flags + (buf * KG + kg) * (4 + RG);
+      const int* flag = flags + (buf * KG + kg) * 4;
       const floatx16 zero16 = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
       floatx16 s[2];
 #pragma unroll
@@ -254,10 +263,6 @@ __global__ __launch_bounds__(64 * RG * KG) __attribute__((amdgpu_waves_per_eu(wa
 #pragma unroll
           for (int i = 0; i < 16; ++i) o[d][i] *= alpha;
       }
-      int nan = 0;
-#pragma unroll
-      for (int w = 0; w < RG; ++w) nan |= flag[4 + w];
-      nan = edge ? __builtin_amdgcn_readfirstlane(nan) : 0;
 #pragma unroll
       for (int c = 0; c < 2; ++c)
 #pragma unroll
@@ -267,37 +272,11 @@ __global__ __launch_bounds__(64 * RG * KG) __attribute__((amdgpu_waves_per_eu(wa
           for (int j = 0; j < 8; ++j) p[j] = s[c][8 * x + j];
           bf16x8 pf[PARTS];
           split<PARTS>(p, pf);
-          if (nan == 0) {
 #pragma unroll
-            for (int d = 0; d < DB; ++d) {
-              const bf16x8 vf = *reinterpret_cast<const bf16x8*>(Vb + min(32 * d + col, DH - 1) * VROW + 32 * c + 16 * x + 8 * g);
+          for (int d = 0; d < DB; ++d) {
+            const bf16x8 vf = *reinterpret_cast<const bf16x8*>(Vb + min(32 * d + col, DH - 1) * VROW + 32 * c + 16 * x + 8 * g);
 #pragma unroll
-              for (int pt = 0; pt < PARTS; ++pt) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, pf[pt], o[d], 0, 0, 0);
-            }
-          } else {
-            // a value that is NaN reaches the rows that read it and no other (its weight of zero would make NaN of the others too): it
-            // is left out of the product, and a second product counts, for every row and dim, the NaN that the row reads
-            float read[8];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) read[j] = reads(c, 8 * x + j) ? 1.f : 0.f;
-            const bf16x8 rf = to_bf16x8(read);
-#pragma unroll
-            for (int d = 0; d < DB; ++d) {
-              const bf16x8 vf = *reinterpret_cast<const bf16x8*>(Vb + min(32 * d + col, DH - 1) * VROW + 32 * c + 16 * x + 8 * g);
-              float clean[8], bad[8];
-#pragma unroll
-              for (int j = 0; j < 8; ++j) {
-                const float v = static_cast<float>(vf[j]);
-                clean[j] = v == v ? v : 0.f;
-                bad[j] = v == v ? 0.f : 1.f;
-              }
-              const bf16x8 cf = to_bf16x8(clean);
-#pragma unroll
-              for (int pt = 0; pt < PARTS; ++pt) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(cf, pf[pt], o[d], 0, 0, 0);
-              const floatx16 n = __builtin_amdgcn_mfma_f32_32x32x16_bf16(to_bf16x8(bad), rf, zero16, 0, 0, 0);
-#pragma unroll
-              for (int i = 0; i < 16; ++i) o[d][i] = n[i] > 0.5f ? NAN : o[d][i];
-            }
+            for (int pt = 0; pt < PARTS; ++pt) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, pf[pt], o[d], 0, 0, 0);
           }
         }
     }
@@ -350,13 +329,39 @@ __global__ __launch_bounds__(64 * RG * KG) __attribute__((amdgpu_waves_per_eu(wa
         }
       }
   }
+  if (*seen != 0 && has_rows) {
+    // a value that is NaN reaches the rows that read it and no other: once more over the values, whose rows' results become NaN in the
+    // value's dim (behind this wave's own stores above)
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup");
+    __builtin_amdgcn_s_waitcnt(0);
+    __builtin_amdgcn_wave_barrier();
+    for (int i = 0; i < steps * KG; ++i) {
+      const int kt = key_of(i / KG) + 64 * (i % KG);
+      for (int x = lane; x < DH * 4; x += 64) {
+        const int dim = x / 4, first = kt + 16 * (x % 4), page = page_of(kt, 16 * (x % 4));
+        if (page < 0) continue;
+        const uint8_t* v = a.v_pool + static_cast<size_t>(page) * page_bytes + (((hk * DH + dim) << a.page_shift) + (first & in_page));
+        for (int j = 0; j < 16; ++j) {
+          if ((v[j] & 0x7f) != 0x7f) continue;
+          const int key = first + j;
+          for (int r = wrow0; r < min(wrow0 + 32, nrows); ++r) {
+            const int pos = pos0 + r;
+            if (key > pos || (key < first_key(pos) && key >= a.keep)) continue;
+            const size_t at = static_cast<size_t>(row0 + r) * a.ldo + h * DH + dim;
+            if (PARTS == 1) static_cast<bf16_t*>(a.out)[at] = bf16_t{0x7fc0};
+            else static_cast<float*>(a.out)[at] = NAN;
+          }
+        }
+      }
+    }
+  }
 }
 
 template <int DH16, int PARTS, int RG, int KG>
 static int launch(const Args& a, int n_tiles, hipStream_t stream) {
   constexpr int DH = DH16 * 16, DB = (DH + 31) / 32;
   constexpr int TILES = 2 * KG * (64 * (DH + 8) + DH * 72) * 2, JOIN = (KG - 1) * 64 * RG * (2 + 16 * DB) * 4;
-  constexpr int BYTES = (TILES > JOIN ? TILES : JOIN) + 2 * KG * (4 + RG) * 4;
+  constexpr int BYTES = (TILES > JOIN ? TILES : JOIN) + 2 * KG * 4 * 4 + 16;
   static_assert(BYTES <= 160 * 1024, "LDS");
   auto* fn = &kernel<DH16, PARTS, RG, KG>;
   if (BYTES > 64 * 1024) {
@@ -395,14 +400,15 @@ extern "C" int dn_attention8_portions(const void* q, int ldq, void* out, int ldo
                                       const int32_t* tile_pos0, int n_tiles, int rows, int groups, int H, int Hkv, int dh, int page_size,
                                       float scale, int window, int keep, int sink, const float* sink_at, float cap, int dtype,
                                       hipStream_t stream) {
-  if (dh < 16 || dh > 256 || dh % 16 != 0 || Hkv < 1 || H % Hkv != 0 || page_size < 16 || page_size % 16 != 0 || !(scale > 0.f) ||
+  if (dh < 16 || dh > 256 || dh % 16 != 0 || Hkv < 1 || H % Hkv != 0 || page_size < 16 || (page_size & (page_size - 1)) != 0 || !(scale > 0.f) ||
+      n_pages < 1 || max_blocks < 1 || static_cast<size_t>(n_pages) * Hkv >= (1ull << 31) || static_cast<size_t>(Hkv) * dh * page_size >= (1ull << 31) ||
       window < 0 || keep < 0 || (keep > 0 && window == 0) || !(cap >= 0.f) || ldq % 8 != 0)
     return DN_ERR_SHAPE;
   if (dtype != DN_F32 && dtype != DN_BF16) return DN_ERR_DTYPE;
   if (n_tiles == 0) return 0;
   const portions8::Args a = {q, out, static_cast<const uint8_t*>(k_pool), static_cast<const uint8_t*>(v_pool), k_scale, v_scale,
                              block_tables, tile_seq, tile_row0, tile_nrows, tile_pos0, sink_at, ldq, ldo, n_pages, max_blocks, H, Hkv,
-                             page_size, window, keep, sink, scale, cap};
+                             __builtin_ctz(page_size), window, keep, sink, scale, cap};
   const int rc = dtype == DN_BF16 ? portions8::by_dim<1>(a, n_tiles, dh, rows, groups, stream)
                                   : portions8::by_dim<3>(a, n_tiles, dh, rows, groups, stream);
   return rc != 0 ? rc : dn_launch_status();

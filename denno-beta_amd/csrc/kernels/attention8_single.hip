@@ -24,7 +24,7 @@ struct Args {
   const int32_t *block_tables, *tile_seq, *tile_row0, *tile_pos0;
   const float* sink_at;
   float* part;      // [tiles][heads][splits][dh + 2]: maximum, sum, weighted values
-  int ldq, ldo, n_pages, max_blocks, n_splits, H, Hkv, page_size, window, keep, sink;
+  int ldq, ldo, n_pages, max_blocks, n_splits, H, Hkv, page_shift, window, keep, sink;      // pages of 1 << page_shift keys
   float scale, cap;
 };
 
@@ -43,7 +43,7 @@ __global__ __launch_bounds__(WAVES * 64) void kernel(const Args a) {
   const int heads = min(G - h0, 16);      // of this workgroup
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64;
   const int c16 = lane % 16, g = lane / 16, kg = c16 / 4;      // column or row; group; the block of this lane's row of keys
-  const int ps = a.page_size;
+  const int in_page = (1 << a.page_shift) - 1;
   const int32_t* bt = a.block_tables + static_cast<size_t>(seq) * a.max_blocks;
 
   // the tiles that the row reads: `kept` ones from the start, then those from the window's first key on; this split's are i0 .. i1
@@ -78,7 +78,7 @@ __global__ __launch_bounds__(WAVES * 64) void kernel(const Args a) {
 
   // the page of the block that begins with `key` and the key's place in it; -1 where the row reads none of it
   auto page_of = [&](int key) {
-    const int b = key / ps;
+    const int b = key >> a.page_shift;
     const int page = key <= pos && b < a.max_blocks ? bt[b] : -1;
     return page < a.n_pages ? page : -1;
   };
@@ -87,15 +87,15 @@ __global__ __launch_bounds__(WAVES * 64) void kernel(const Args a) {
     const int kb = kt + 16 * kg, vb = kt + 16 * g;
     const int k_page = page_of(kb), v_page = page_of(vb);
     const size_t kph = static_cast<size_t>(max(k_page, 0)) * a.Hkv + hk, vph = static_cast<size_t>(max(v_page, 0)) * a.Hkv + hk;
-    const uint8_t* kp = a.k_pool + (kph * ps + kb % ps + c16 % 4) * DH + g * 16;
-    const uint8_t* vp = a.v_pool + (vph * DH + c16) * ps + vb % ps;
+    const uint8_t* kp = a.k_pool + ((kph << a.page_shift) + (kb & in_page) + c16 % 4) * DH + g * 16;
+    const uint8_t* vp = a.v_pool + ((vph * DH + c16) << a.page_shift) + (vb & in_page);
     u32x4 kr[4][NC], vr[DH16];
 #pragma unroll
     for (int t = 0; t < 4; ++t)
 #pragma unroll
       for (int c = 0; c < NC; ++c) kr[t][c] = *reinterpret_cast<const u32x4*>(kp + t * 4 * DH + (4 * c + g < DH16 ? c * 64 : -g * 16));
 #pragma unroll
-    for (int d = 0; d < DH16; ++d) vr[d] = *reinterpret_cast<const u32x4*>(vp + static_cast<size_t>(d) * 16 * ps);
+    for (int d = 0; d < DH16; ++d) vr[d] = *reinterpret_cast<const u32x4*>(vp + (static_cast<size_t>(d) * 16 << a.page_shift));
     const float ks = a.k_scale[vph] * scale2, vs = a.v_scale[vph];
 
     floatx4 s[4];
@@ -279,14 +279,14 @@ extern "C" int dn_attention8_single(const void* q, int ldq, void* out, int ldo, 
                                     const int32_t* tile_seq, const int32_t* tile_row0, const int32_t* tile_pos0, int n_tiles, float* part,
                                     int n_splits, int waves, int H, int Hkv, int dh, int page_size, float scale, int window, int keep,
                                     int sink, const float* sink_at, float cap, int dtype, hipStream_t stream) {
-  if (dh < 16 || dh > 256 || dh % 16 != 0 || Hkv < 1 || H % Hkv != 0 || page_size < 16 || page_size % 16 != 0 || window < 0 || keep < 0 ||
+  if (dh < 16 || dh > 256 || dh % 16 != 0 || Hkv < 1 || H % Hkv != 0 || page_size < 16 || (page_size & (page_size - 1)) != 0 || window < 0 || keep < 0 ||
       (keep > 0 && window == 0) || !(cap >= 0.f) || n_splits < 1 || (n_splits > 1 && !part))
     return DN_ERR_SHAPE;
   if (dtype != DN_F32 && dtype != DN_BF16) return DN_ERR_DTYPE;
   if (n_tiles == 0) return 0;
   const single8::Args a = {q, out, static_cast<const uint8_t*>(k_pool), static_cast<const uint8_t*>(v_pool), k_scale, v_scale,
                            block_tables, tile_seq, tile_row0, tile_pos0, sink_at, part, ldq, ldo, n_pages, max_blocks, n_splits, H, Hkv,
-                           page_size, window, keep, sink, scale, cap};
+                           __builtin_ctz(page_size), window, keep, sink, scale, cap};
   const int rc = dtype == DN_BF16 ? single8::by_dim<1>(a, n_tiles, dh, waves, stream) : single8::by_dim<3>(a, n_tiles, dh, waves, stream);
   if (rc != 0) return rc;
   if (n_splits > 1) {

@@ -1066,7 +1066,8 @@ def attention8(q, out, k_pool, v_pool, k_scale, v_scale, block_tables, tiles, n_
     if T == 0 or n_tiles == 0:
         return out
     base = tiles.data_ptr()
-    aligned = (dh % 16 == 0 and ps % 16 == 0 and k_pool.data_ptr() % 16 == 0 and v_pool.data_ptr() % 16 == 0)
+    # (the kernels on the matrix cores: heads of a multiple of 16, pages of a power of two from 16 keys on)
+    aligned = (dh % 16 == 0 and ps >= 16 and ps & (ps - 1) == 0 and k_pool.data_ptr() % 16 == 0 and v_pool.data_ptr() % 16 == 0)
     if single_rows and max_context > 0:
         _need(n_tiles == T, "attention8: a step of single rows has a tile for every row")
         _need(max_context <= block_tables.shape[1] * ps, "attention8: max_context exceeds the block tables")
