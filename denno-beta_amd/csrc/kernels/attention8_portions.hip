@@ -132,26 +132,28 @@ __global__ __launch_bounds__(64 * RG * KG) __attribute__((amdgpu_waves_per_eu(wa
     k_at[u] = ((hk << a.page_shift) + (k_key[u] & in_page)) * DH + x % DH16 * 16;
     v_at[u] = ((hk * DH + x / 4) << a.page_shift) + (v_block & in_page);
   }
-  // the page of the block of 16 keys that key kt + off stands in (off < 64); -1: none, or behind the last row
-  auto page_of = [&](int kt, int off) {
-    const int b = (kt >> a.page_shift) + (off >> a.page_shift);
-    const int page = bt[min(b, a.max_blocks - 1)];
-    return b < a.max_blocks && kt + (off & ~15) <= hi_g && page < a.n_pages ? page : -1;
+  // The page of the block of 16 keys that key kt + off stands in (off < 64): what the table says is asked for a step before it is
+  // needed (page_entry), and judged when it is (page_of; -1: none, or behind the last row): judged at once, it would be waited for at
+  // once, and with it the keys and values on their way.
+  auto page_entry = [&](int kt, int off) { return bt[min((kt >> a.page_shift) + (off >> a.page_shift), a.max_blocks - 1)]; };
+  auto page_of = [&](int kt, int off, int entry) {
+    return (kt >> a.page_shift) + (off >> a.page_shift) < a.max_blocks && kt + (off & ~15) <= hi_g && entry < a.n_pages ? entry : -1;
   };
   auto pages = [&](int i) {
     const int kt = key_of(i) + 64 * kg;      // (a step behind the last one begins behind the last row)
 #pragma unroll
-    for (int u = 0; u < U; ++u) k_page[u] = page_of(kt, k_key[u]);
-    v_page = page_of(kt, v_block);
+    for (int u = 0; u < U; ++u) k_page[u] = page_entry(kt, k_key[u]);
+    v_page = page_entry(kt, v_block);
   };
   auto fetch = [&](int i) {      // (what has no page reads the pools' first: no row reads what comes of it)
     const int kt = key_of(i) + 64 * kg, far = kt & in_page;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const uint32_t page = max(k_page[u], 0);
+      const uint32_t page = max(page_of(kt, k_key[u], k_page[u]), 0);
       k_raw[u] = *reinterpret_cast<const u32x4*>(a.k_pool + static_cast<size_t>(page) * page_bytes + (k_at[u] + far * DH));
       k_by[u] = a.k_scale[page * a.Hkv + hk];
     }
+    v_page = page_of(kt, v_block, v_page);
     const uint32_t page = max(v_page, 0);
     v_by = a.v_scale[page * a.Hkv + hk];
     v_there = v_page >= 0;
@@ -209,18 +211,39 @@ __global__ __launch_bounds__(64 * RG * KG) __attribute__((amdgpu_waves_per_eu(wa
       const bf16_t* Vb = Kb + KSZ;
       const int* flag = flags + (buf * KG + kg) * 4;
       const floatx16 zero16 = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+      const u32x4 there4 = *reinterpret_cast<const u32x4*>(flag);      // blocks with a page
+      // The operands that LDS gives come four at a time, one such group ahead of the products (a read takes as long as three or four
+      // products), the values' first group while the softmax is made.
+      auto key_part = [&](int f) { return *reinterpret_cast<const bf16x8*>(Kb + (32 * (f / DH16) + col) * KROW + f % DH16 * 16 + g * 8); };
+      auto value_part = [&](int f) {      // f: block of 16 keys, then of 32 dims
+        return *reinterpret_cast<const bf16x8*>(Vb + min(32 * (f % DB) + col, DH - 1) * VROW + 16 * (f / DB) + 8 * g);
+      };
+      constexpr int KF = 2 * DH16, VF = 4 * DB;
+      bf16x8 part[2][4];
       floatx16 s[2];
 #pragma unroll
-      for (int c = 0; c < 2; ++c)
+      for (int j = 0; j < 4; ++j)
+        if (j < KF) part[0][j] = key_part(j);
 #pragma unroll
-        for (int d = 0; d < DH16; ++d) {
-          const bf16x8 kf = *reinterpret_cast<const bf16x8*>(Kb + (32 * c + col) * KROW + d * 16 + g * 8);
+      for (int f = 0; f < KF; f += 4) {
 #pragma unroll
-          for (int p = 0; p < PARTS; ++p) s[c] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, qf[d][p], d == 0 && p == 0 ? zero16 : s[c], 0, 0, 0);
+        for (int j = 0; j < 4; ++j) {
+          if (f + 4 + j < KF) part[(f / 4 + 1) % 2][j] = key_part(f + 4 + j);
+          else if (f + 4 >= KF && j < VF) part[(f / 4 + 1) % 2][j] = value_part(j);
         }
-      // s[c][i]: key kw + 32 c + 8 (i / 4) + 4 g + i % 4 of this lane's row
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (f + j < KF) {
+            const int c = (f + j) / DH16, d = (f + j) % DH16;
+#pragma unroll
+            for (int p = 0; p < PARTS; ++p)
+              s[c] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(part[f / 4 % 2][j], qf[d][p], d == 0 && p == 0 ? zero16 : s[c], 0, 0, 0);
+          }
+        __builtin_amdgcn_sched_barrier(0);
+      }
       settle(s[0], s[1]);
-      const int there = __builtin_amdgcn_readfirstlane(flag[0] | flag[1] << 1 | flag[2] << 2 | flag[3] << 3);      // blocks with a page
+      const int there = __builtin_amdgcn_readfirstlane(there4[0] | there4[1] << 1 | there4[2] << 2 | there4[3] << 3);
       // an edge: a key that one of the wave's rows does not read.  The same for the whole wave.
       const bool edge = kw + 63 > pos0 + wrow0 || (kw < lo_last && kw + 63 >= a.keep) || there != 15;
       // whether this lane's row reads its i-th key of the half tile c (no branches: all of it is one comparison after the other)
@@ -240,45 +263,53 @@ __global__ __launch_bounds__(64 * RG * KG) __attribute__((amdgpu_waves_per_eu(wa
 #pragma unroll
           for (int i = 0; i < 16; ++i) s[c][i] = reads(c, i) ? s[c][i] : -INFINITY;
       }
-      float top = LOWEST;
+      float top = LOWEST, tops[4] = {LOWEST, LOWEST, LOWEST, LOWEST};
 #pragma unroll
-      for (int c = 0; c < 2; ++c)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) top = fmaxf(top, s[c][i]);
+      for (int i = 0; i < 16; ++i) tops[i % 4] = fmaxf(fmaxf(tops[i % 4], s[0][i]), s[1][i]);
+      top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
       top = fmaxf(top, other_half(top));
       const float m_new = fmaxf(m_run, top * per_score), alpha = __builtin_amdgcn_exp2f(m_run - m_new);
       m_run = m_new;
-      float sum = 0.f;
+      float sums[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int c = 0; c < 2; ++c)
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
           s[c][i] = __builtin_amdgcn_exp2f(fmaf(s[c][i], per_score, -m_new));
-          sum += s[c][i];
+          sums[i % 4] += s[c][i];
         }
-      l_run = l_run * alpha + sum;
+      l_run = l_run * alpha + ((sums[0] + sums[1]) + (sums[2] + sums[3]));
       if (__builtin_amdgcn_ballot_w64(alpha != 1.f) != 0) {
 #pragma unroll
         for (int d = 0; d < DB; ++d)
 #pragma unroll
           for (int i = 0; i < 16; ++i) o[d][i] *= alpha;
       }
+      bf16x8 pf[4][PARTS];
 #pragma unroll
-      for (int c = 0; c < 2; ++c)
+      for (int x = 0; x < 4; ++x) {
+        float p[8];
 #pragma unroll
-        for (int x = 0; x < 2; ++x) {
-          float p[8];
+        for (int j = 0; j < 8; ++j) p[j] = s[x / 2][8 * (x % 2) + j];
+        split<PARTS>(p, pf[x]);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      constexpr int V0 = (KF + 3) / 4;      // the group of `part` that the values begin in
 #pragma unroll
-          for (int j = 0; j < 8; ++j) p[j] = s[c][8 * x + j];
-          bf16x8 pf[PARTS];
-          split<PARTS>(p, pf);
+      for (int f = 0; f < VF; f += 4) {
 #pragma unroll
-          for (int d = 0; d < DB; ++d) {
-            const bf16x8 vf = *reinterpret_cast<const bf16x8*>(Vb + min(32 * d + col, DH - 1) * VROW + 32 * c + 16 * x + 8 * g);
+        for (int j = 0; j < 4; ++j)
+          if (f + 4 + j < VF) part[(V0 + f / 4 + 1) % 2][j] = value_part(f + 4 + j);
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int pt = 0; pt < PARTS; ++pt) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, pf[pt], o[d], 0, 0, 0);
+        for (int j = 0; j < 4; ++j)
+          if (f + j < VF) {
+            const int x = (f + j) / DB, d = (f + j) % DB;
+#pragma unroll
+            for (int pt = 0; pt < PARTS; ++pt) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(part[(V0 + f / 4) % 2][j], pf[x][pt], o[d], 0, 0, 0);
           }
-        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
     }
     __syncthreads();
   }
@@ -338,7 +369,7 @@ __global__ __launch_bounds__(64 * RG * KG) __attribute__((amdgpu_waves_per_eu(wa
     for (int i = 0; i < steps * KG; ++i) {
       const int kt = key_of(i / KG) + 64 * (i % KG);
       for (int x = lane; x < DH * 4; x += 64) {
-        const int dim = x / 4, first = kt + 16 * (x % 4), page = page_of(kt, 16 * (x % 4));
+        const int dim = x / 4, first = kt + 16 * (x % 4), page = page_of(kt, 16 * (x % 4), page_entry(kt, 16 * (x % 4)));
         if (page < 0) continue;
         const uint8_t* v = a.v_pool + static_cast<size_t>(page) * page_bytes + (((hk * DH + dim) << a.page_shift) + (first & in_page));
         for (int j = 0; j < 16; ++j) {
