@@ -114,23 +114,23 @@ __global__ __launch_bounds__(64 * RG * KG) __attribute__((amdgpu_waves_per_eu(wa
   const int steps = kept + max(0, hi_g / STEP - rest + 1);
   auto key_of = [&](int i) { return STEP * (i < kept ? i : rest + i - kept); };
 
-  // This thread's chunks of its group's tile: chunk x = t + THREADS u is, of the keys, 16 dims (x % DH16) of key x / DH16; of the
-  // values, the 16 keys of block x % 4 of dim x / 4 (the same block for every u).  A tile begins at a multiple of 64, so in pages of up to
-  // 64 keys a chunk's place in its page is always the same, and in longer ones what is added to it is the same for all threads.
+  // This thread's chunks of its group's tile are all of block t % 4, its 16 keys, so that a thread has one page a tile: chunk x = t / 4 +
+  // THREADS / 4 u is, of the keys, 16 dims (x % DH16) of key x / DH16, and of the values dim x.  A tile begins at a multiple of 64, so in
+  // pages of up to 64 keys a block's place in its page is always the same, and in longer ones what is added to it is the same for all threads.
+  constexpr int BLOCK_CHUNKS = CHUNKS / 4;
   const int in_page = (1 << a.page_shift) - 1;
   const uint32_t page_bytes = static_cast<uint32_t>(a.Hkv) * DH << a.page_shift;
-  int k_key[U], k_page[U], v_page;
+  const int off = 16 * (t % 4);
+  int entry;                     // what the table says of the block's page, a step before it is needed
   uint32_t k_at[U], v_at[U];
   u32x4 k_raw[U], v_raw[U];
-  float k_by[U], v_by;
-  bool v_there = false;      // whether the values in registers have a page
-  const int v_block = 16 * (t % 4);
+  float k_by, v_by;
+  bool there_is = false;         // whether what is in registers has a page
 #pragma unroll
   for (int u = 0; u < U; ++u) {
-    const int x = min(t + THREADS * u, CHUNKS - 1);
-    k_key[u] = x / DH16;
-    k_at[u] = ((hk << a.page_shift) + (k_key[u] & in_page)) * DH + x % DH16 * 16;
-    v_at[u] = ((hk * DH + x / 4) << a.page_shift) + (v_block & in_page);
+    const int x = min(t / 4 + THREADS / 4 * u, BLOCK_CHUNKS - 1);
+    k_at[u] = ((hk << a.page_shift) + (off & in_page) + x / DH16) * DH + x % DH16 * 16;
+    v_at[u] = ((hk * DH + x) << a.page_shift) + (off & in_page);
   }
   // The page of the block of 16 keys that key kt + off stands in (off < 64): what the table says is asked for a step before it is
   // needed (page_entry), and judged when it is (page_of; -1: none, or behind the last row): judged at once, it would be waited for at
@@ -139,26 +139,19 @@ __global__ __launch_bounds__(64 * RG * KG) __attribute__((amdgpu_waves_per_eu(wa
   auto page_of = [&](int kt, int off, int entry) {
     return (kt >> a.page_shift) + (off >> a.page_shift) < a.max_blocks && kt + (off & ~15) <= hi_g && entry < a.n_pages ? entry : -1;
   };
-  auto pages = [&](int i) {
-    const int kt = key_of(i) + 64 * kg;      // (a step behind the last one begins behind the last row)
-#pragma unroll
-    for (int u = 0; u < U; ++u) k_page[u] = page_entry(kt, k_key[u]);
-    v_page = page_entry(kt, v_block);
-  };
+  auto pages = [&](int i) { entry = page_entry(key_of(i) + 64 * kg, off); };      // (a step behind the last one begins behind the last row)
   auto fetch = [&](int i) {      // (what has no page reads the pools' first: no row reads what comes of it)
-    const int kt = key_of(i) + 64 * kg, far = kt & in_page;
+    const int kt = key_of(i) + 64 * kg, far = kt & in_page, judged = page_of(kt, off, entry);
+    const uint32_t page = max(judged, 0);
+    there_is = judged >= 0;
+    const size_t begin = static_cast<size_t>(page) * page_bytes;
+    k_by = a.k_scale[page * a.Hkv + hk];
+    v_by = a.v_scale[page * a.Hkv + hk];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const uint32_t page = max(page_of(kt, k_key[u], k_page[u]), 0);
-      k_raw[u] = *reinterpret_cast<const u32x4*>(a.k_pool + static_cast<size_t>(page) * page_bytes + (k_at[u] + far * DH));
-      k_by[u] = a.k_scale[page * a.Hkv + hk];
+      k_raw[u] = *reinterpret_cast<const u32x4*>(a.k_pool + begin + (k_at[u] + far * DH));
+      v_raw[u] = *reinterpret_cast<const u32x4*>(a.v_pool + begin + (v_at[u] + far));
     }
-    v_page = page_of(kt, v_block, v_page);
-    const uint32_t page = max(v_page, 0);
-    v_by = a.v_scale[page * a.Hkv + hk];
-    v_there = v_page >= 0;
-#pragma unroll
-    for (int u = 0; u < U; ++u) v_raw[u] = *reinterpret_cast<const u32x4*>(a.v_pool + static_cast<size_t>(page) * page_bytes + (v_at[u] + far));
   };
   auto stash = [&](int i, int buf) {
     bf16_t* dst = tiles + (buf * KG + kg) * TSZ;
@@ -172,21 +165,21 @@ __global__ __launch_bounds__(64 * RG * KG) __attribute__((amdgpu_waves_per_eu(wa
       for (int u = 0; u < U; ++u)
 #pragma unroll
         for (int w = 0; w < 4; ++w) v_raw[u][w] &= ~((nan_in(v_raw[u][w]) >> 7) * 0xffu);
-      if (nan != 0 && v_there) *seen = 1;
+      if (nan != 0 && there_is) *seen = 1;
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int x = t + THREADS * u;
-      if (CHUNKS % THREADS == 0 || x < CHUNKS) {
-        u32x4* to = reinterpret_cast<u32x4*>(dst + x / DH16 * KROW + x % DH16 * 16);
-        to[0] = widen_scaled(k_raw[u][0], k_raw[u][1], k_by[u]);
-        to[1] = widen_scaled(k_raw[u][2], k_raw[u][3], k_by[u]);
-        to = reinterpret_cast<u32x4*>(dst + KSZ + x / 4 * VROW + x % 4 * 16);
+      const int x = t / 4 + THREADS / 4 * u;
+      if (CHUNKS % THREADS == 0 || x < BLOCK_CHUNKS) {
+        u32x4* to = reinterpret_cast<u32x4*>(dst + (off + x / DH16) * KROW + x % DH16 * 16);
+        to[0] = widen_scaled(k_raw[u][0], k_raw[u][1], k_by);
+        to[1] = widen_scaled(k_raw[u][2], k_raw[u][3], k_by);
+        to = reinterpret_cast<u32x4*>(dst + KSZ + x * VROW + off);
         to[0] = widen_scaled(v_raw[u][0], v_raw[u][2], v_by);
         to[1] = widen_scaled(v_raw[u][1], v_raw[u][3], v_by);
       }
     }
-    if (t < 4) flags[(buf * KG + kg) * 4 + t] = v_there;
+    if (t < 4) flags[(buf * KG + kg) * 4 + t] = there_is;
   };
 
   if (threadIdx.x == 0) *seen = 0;

@@ -1010,9 +1010,16 @@ def _single8_shape(n_tiles, n_heads, Hkv, dh, max_context, window, keep_first):
     return waves, max(1, min(-(-reach // 64) // (2 * waves), 256 // groups))
 
 
-def _portions8_shape(n_tiles, n_heads, dh):
-    """-> (groups of 32 rows, groups of keys) of a workgroup of the portions' kernel."""
-    return 4, 1
+def _portions8_shape(n_tiles, n_heads, dh, dtype):
+    """-> (groups of 32 rows, groups of keys) of a workgroup of the portions' kernel.  Where tiles of 128 rows alone give the chip less than a
+    workgroup per CU, halves of them, whose keys two groups share out (a row's time is the keys that its wave walks): 1,001 rows, 25 heads of
+    64, 20.0 us, undivided 26.7.  Up to two and a half per CU the keys only: 2,048 rows 26.1 and 29.3, 2,012 rows of 32 heads of 128
+    behind 2,001 to 8,192 tokens 288 and 301.  Beyond that neither: 4,000 rows behind 1,000 tokens 92 us, with keys shared out 113.  What
+    does not fit the registers so (heads beyond 128; 32-bit ones beyond 96, bfloat16 ones beyond 96 in halves) goes the next best way."""
+    blocks = n_tiles * n_heads
+    if dh > (128 if dtype is torch.bfloat16 else 96) or blocks > 640:
+        return 4, 1
+    return (2, 2) if blocks <= 256 and dh <= 96 else (4, 2)
 
 
 def _attention8_holds(q, out, block_tables, tiles, n_heads, Hkv, dh):
@@ -1085,7 +1092,7 @@ def attention8(q, out, k_pool, v_pool, k_scale, v_scale, block_tables, tiles, n_
         _dev(tiles_wide, "tiles_wide", _I32, 2)
         _need(tiles_wide.is_contiguous() and tiles_wide.shape[0] == 4, "attention8: tiles_wide")
         n_wide = tiles_wide.shape[1]
-        rows, groups = _portions8_shape(n_wide, n_heads, dh)
+        rows, groups = _portions8_shape(n_wide, n_heads, dh, q.dtype)
         base = tiles_wide.data_ptr()
         _ok(_lib("cache8").dn_attention8_portions(
             q.data_ptr(), ldq, out.data_ptr(), ldo, k_pool.data_ptr(), v_pool.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),

@@ -360,3 +360,163 @@ def test_attention_rows_that_read_nothing_and_padding(dtype):
         ops().attention8(q.to(DEV), sunk, *[p.to(DEV) for p in pools], bt.to(DEV), tiles.to(DEV), H, dh ** -0.5, tiles_wide=wide.to(DEV),
                          single_rows=single, max_context=60, sink=True)
         assert bool((sunk[row - 1] == 0).all())
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("H,hkv,dh", [(4, 2, 16), (2, 2, 64), (4, 1, 80), (3, 3, 128)])
+@pytest.mark.parametrize("shape", [(4, 1), (4, 2), (2, 2)], ids=str)
+def test_attention_portions_in_every_shape(monkeypatch, dtype, H, hkv, dh, shape):
+    """Every shape of workgroup of the portions' kernel, not only the one that its rule picks for this little work."""
+    o = ops()
+    monkeypatch.setattr(o, "_portions8_shape", lambda *a: shape)
+    kw = dict(window=150, keep_first=5, sink=True) if dh == 64 else dict(softcap=10.0) if dh == 80 else {}
+    case = attention_case([300, 260, 133, 65], [1, 260, 21, 33], H, hkv, dh, 16, dtype, seed=dh, window=kw.get("window", 0), keep=kw.get("keep_first", 0))
+    check_attention(*case, H, dh ** -0.5, dtype, what=shape, **kw)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("H,hkv,dh", [(4, 2, 16), (40, 2, 64), (3, 3, 128), (2, 1, 208)])
+@pytest.mark.parametrize("waves,splits", [(4, 1), (4, 3), (8, 1), (8, 2), (4, 20)])
+def test_attention_single_rows_in_every_shape(monkeypatch, dtype, H, hkv, dh, waves, splits):
+    """Every number of waves and of workgroups that share a row's keys out, more workgroups than tiles of keys among them."""
+    if waves == 8 and dh > 128:
+        pytest.skip("heads beyond 128 go in workgroups of four waves")
+    o = ops()
+    monkeypatch.setattr(o, "_single8_shape", lambda *a: (waves, splits))
+    kw = dict(window=150, keep_first=5, sink=True) if dh == 64 else {}
+    lens = [700, 1, 64, 300]
+    case = attention_case(lens, [1] * 4, H, hkv, dh, 16, dtype, seed=dh, window=kw.get("window", 0), keep=kw.get("keep_first", 0))
+    check_attention(*case, H, dh ** -0.5, dtype, single=True, longest=700, what=(waves, splits), **kw)
+
+
+def test_attention_shapes_are_refused_by_the_entries():
+    o = ops()
+    q = torch.zeros(1, 256, dtype=BF16, device=DEV)
+    p = [t.to(DEV) for t in random_pools(2, 1, 16, 256, torch.Generator().manual_seed(0))]
+    bt, tiles = torch.zeros(1, 1, dtype=torch.int32, device=DEV), i32([[0], [0], [1], [0]]).to(DEV)
+    for name, shape, kw in (("_single8_shape", (8, 1), dict(single_rows=True, max_context=1)), ("_portions8_shape", (2, 2), dict(tiles_wide=tiles))):
+        real = getattr(o, name)
+        setattr(o, name, lambda *a: shape)
+        try:
+            with pytest.raises(o.KernelError, match="sizes"):
+                o.attention8(q, torch.empty_like(q), *p, bt, tiles, 1, 1.0, **kw)
+        finally:
+            setattr(o, name, real)
+
+
+def test_attention_scales_that_are_not_positive():
+    """A scale below zero (the portions' kernel takes the largest product for the largest score: it goes the plain way) and zero."""
+    case = attention_case([100, 70], [40, 70], 4, 2, 64, 16, BF16, seed=12)
+    for scale in (-0.125, 0.0):
+        q, pools, bt, tiles, wide = case
+        want, mass, most = R.attention_exact(q, *pools, bt, tiles, 4, scale)
+        got = torch.empty(q.shape[0], 256, dtype=BF16, device=DEV)
+        ops().attention8(q.to(DEV), got, *[p.to(DEV) for p in pools], bt.to(DEV), tiles.to(DEV), 4, scale, tiles_wide=wide.to(DEV))
+        loss = 2.0 ** -23 + 2 * 72 * 2.0 ** -23 * most.abs().repeat_interleave(64, 1) + 2 * 128 * 2.0 ** -24
+        assert bool(((got.cpu().double() - want).abs() <= 2.0 ** -8 * want.abs() + loss * mass * 1.01 + 1e-30).all())
+
+
+def test_calls_on_another_stream_and_two_at_once():
+    """Two streams that use the operators at once, each on tensors of its own, get what one after the other gives."""
+    gen = torch.Generator().manual_seed(13)
+    hkv, dh, ps, H = 4, 64, 16, 8
+    lens = [900, 33, 517]
+
+    def state(seed):
+        q, pools, bt, tiles, wide = attention_case(lens, [1] * 3, H, hkv, dh, ps, BF16, seed=seed)
+        src = torch.randn(3, 2 * hkv * dh, generator=gen).to(BF16).to(DEV)
+        slots = i32([int(bt[s, (n - 1) // ps]) * ps + (n - 1) % ps for s, n in enumerate(lens)]).to(DEV)
+        return [t.to(DEV) for t in (q, bt, tiles)], [p.to(DEV) for p in pools], src, slots
+
+    def run(st):
+        (q, bt, tiles), pools, src, slots = st
+        out = []
+        for _ in range(20):
+            ops().kv_append8(src, 0, hkv * dh, slots, *pools)
+            out.append(ops().attention8(q, torch.empty_like(q), *pools, bt, tiles, H, 0.125, single_rows=True, max_context=900))
+        return out
+    states = [state(20), state(21)]
+    want = [run((s[0], [p.clone() for p in s[1]], *s[2:])) for s in states]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in states]
+    got = []
+    for st, stream in zip(states, streams):
+        with torch.cuda.stream(stream):
+            got.append(run(st))
+    torch.cuda.synchronize()
+    for a, b in zip(got, want):
+        for x, y in zip(a, b):
+            assert torch.equal(x, y)
+
+
+def test_two_captured_graphs_of_a_step():
+    """Append and attention captured together, twice over different caches; the graphs are replayed in turn with eager work and
+    synchronizations between them, and every replay gives the eager result (the split results' workspaces are the graphs' own)."""
+    hkv, dh, ps, H = 2, 128, 16, 8
+
+    def state(seed, n):
+        q, pools, bt, tiles, wide = attention_case([n], [1], H, hkv, dh, ps, BF16, seed=seed)
+        src = torch.randn(1, (H + 2 * hkv) * dh, generator=torch.Generator().manual_seed(seed)).to(BF16)
+        slot = i32([int(bt[0, (n - 1) // ps]) * ps + (n - 1) % ps])
+        freq = (10000.0 ** (-torch.arange(dh // 2).double() * 2 / dh)).float()
+        return [t.to(DEV) for t in (src, slot, i32([n - 1]), freq, bt, tiles)], [p.to(DEV) for p in pools], n
+
+    def step(st, pools):
+        (src, slot, pos, freq, bt, tiles), _, n = st
+        turned = torch.empty(1, H * dh, dtype=BF16, device=DEV)
+        ops().kv_append8(src, H * dh, (H + hkv) * dh, slot, *pools, positions=pos, freq=freq, q_out=turned, q_col=0, n_heads=H)
+        return ops().attention8(turned, torch.empty_like(turned), *pools, bt, tiles, H, dh ** -0.5, single_rows=True, max_context=n)
+    states = [state(31, 6000), state(32, 4100)]
+    want = [step(s, [p.clone() for p in s[1]]) for s in states]
+    assert ops()._single8_shape(1, H, hkv, dh, 6000, 0, 0)[1] > 1
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for s in states:
+            step(s, [p.clone() for p in s[1]])
+    torch.cuda.current_stream().wait_stream(side)
+    graphs, outs = [], []
+    for s in states:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(step(s, s[1]))
+        graphs.append(g)
+    for turn in range(4):
+        for g in graphs:
+            g.replay()
+        torch.cuda.synchronize()
+        x = torch.randn(256, 256, device=DEV)
+        (x @ x).sum().item()
+        for a, b in zip(outs, want):
+            assert torch.equal(a, b), turn
+
+
+def test_long_caches_pass_32_bits():
+    """Pools of more than 2^31 numbers, the pages at their end."""
+    hkv, dh, ps, H = 2, 256, 16, 4
+    n_pages = (1 << 31) // (hkv * ps * dh) + 40
+    k = torch.zeros(n_pages, hkv, ps, dh, dtype=torch.uint8, device=DEV).view(FP8)
+    v = torch.zeros(n_pages, hkv, dh, ps, dtype=torch.uint8, device=DEV).view(FP8)
+    ks, vs = torch.ones(n_pages, hkv, device=DEV), torch.ones(n_pages, hkv, device=DEV)
+    gen = torch.Generator().manual_seed(14)
+    n = 40
+    pages = [n_pages - 1, n_pages - 17, n_pages - 30]
+    src = torch.randn(n, (H + 2 * hkv) * dh, generator=gen).to(BF16)
+    slots = i32([pages[i // ps] * ps + i % ps for i in range(n)])
+    ops().kv_append8(src.to(DEV), H * dh, (H + hkv) * dh, slots.to(DEV), k, v, ks, vs)
+    small = [torch.zeros(3, hkv, ps, dh, dtype=FP8), torch.zeros(3, hkv, dh, ps, dtype=FP8), torch.zeros(3, hkv), torch.zeros(3, hkv)]
+    R.kv_append8(src, H * dh, (H + hkv) * dh, i32(range(n)), *small)
+    for big, want in zip((k, v, ks, vs), small):
+        assert same(torch.stack([big[p] for p in pages]), want)
+    bt, tiles = i32([pages]), i32([[0, 0, 0], [0, 16, 32], [16, 16, 8], [0, 16, 32]])
+    wide = i32([[0], [0], [n], [0]])
+    q = src[:, :H * dh].contiguous()
+    want, _, _ = R.attention_exact(q, *small, i32([[0, 1, 2]]), tiles, H, 0.0625)
+    for dtype in (BF16, F32):
+        for kw in (dict(tiles_wide=wide.to(DEV)), dict()):
+            got = ops().attention8(q.to(dtype).to(DEV), torch.empty(n, H * dh, dtype=dtype, device=DEV), k, v, ks, vs, bt.to(DEV), tiles.to(DEV), H, 0.0625, **kw)
+            assert torch.allclose(got.cpu().double(), want, atol=0.03, rtol=0.02)
+        one = i32([[0], [0], [1], [n - 1]]).to(DEV)
+        got = ops().attention8(q[n - 1:].to(dtype).to(DEV), torch.empty(1, H * dh, dtype=dtype, device=DEV), k, v, ks, vs, bt.to(DEV), one, H, 0.0625,
+                               single_rows=True, max_context=n)
+        assert torch.allclose(got.cpu().double(), want[n - 1:], atol=0.03, rtol=0.02)
