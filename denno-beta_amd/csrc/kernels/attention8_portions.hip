@@ -66,8 +66,19 @@ __global__ __launch_bounds__(64 * RG * KG) __attribute__((amdgpu_waves_per_eu(wa
   // consecutive workgroups go to different XCDs: the heads of one key head are Hkv workgroups apart, so that with 8 key heads (or a
   // multiple) an XCD's L2 holds the keys of its own heads only
   const int G = a.H / a.Hkv;
-  const int hk = blockIdx.x % a.Hkv, h = hk * G + blockIdx.x / a.Hkv;
-  const int tile = blockIdx.y / SUBS, sub = SUBS - 1 - blockIdx.y % SUBS;      // (the longest first)
+  // Tiles come with the longest first.  The first 256 workgroups go to a CU each, and the next 256 to the same CUs in the same order: those
+  // are taken the other way round (in eights, which go to the eight XCDs), so that the longest have the shortest beside them (two prompts
+  // of 1,024 with 25 heads of 64: 28.3 -> 26.8 us; workgroups of 8 waves, of which a CU holds one, wait for a free CU and stay in order).
+  int bx = blockIdx.x, by = blockIdx.y;
+  if constexpr (RG == 2) {
+    const int b = by * gridDim.x + bx, eights = gridDim.x * gridDim.y / 8, end = min(eights, 64);
+    if (b >= 256 && b / 8 < end) {
+      const int other = (32 + end - 1 - b / 8) * 8 + b % 8;
+      by = other / gridDim.x, bx = other % gridDim.x;
+    }
+  }
+  const int hk = bx % a.Hkv, h = hk * G + bx / a.Hkv;
+  const int tile = by / SUBS, sub = SUBS - 1 - by % SUBS;
   const int seq = a.tile_seq[tile];
   const int r0 = sub * 32 * RG;
   const int nrows = min(a.tile_nrows[tile] - r0, 32 * RG);
@@ -121,14 +132,19 @@ __global__ __launch_bounds__(64 * RG * KG) __attribute__((amdgpu_waves_per_eu(wa
   const int in_page = (1 << a.page_shift) - 1;
   const uint32_t page_bytes = static_cast<uint32_t>(a.Hkv) * DH << a.page_shift;
   const int off = 16 * (t % 4);
-  int entry;                     // what the table says of the block's page, a step before it is needed
-  uint32_t k_at[U], v_at[U];
-  u32x4 k_raw[U], v_raw[U];
-  float k_by, v_by;
-  bool there_is = false;         // whether what is in registers has a page
+  // (the chunks of one thread lie evenly apart if a group's threads take whole keys at a time: one place to keep then)
+  constexpr bool EVEN = CHUNKS % THREADS == 0 && THREADS / 4 % DH16 == 0;
+  constexpr int PLACES = EVEN ? 1 : U;
+  uint32_t k_at[PLACES], v_at[PLACES];
+  struct Raw {                   // a tile on its way
+    u32x4 k[U], v[U];
+    float k_by, v_by;
+    bool there;                  // whether it has a page
+  };
 #pragma unroll
-  for (int u = 0; u < U; ++u) {
-    const int x = min(t / 4 + THREADS / 4 * u, BLOCK_CHUNKS - 1);
+  for (int u = 0; u < PLACES; ++u) {
+    // (a thread without a chunk takes another's)
+    const uint32_t x = CHUNKS % THREADS == 0 ? t / 4 + THREADS / 4 * u : min(t / 4 + THREADS / 4 * u, BLOCK_CHUNKS - 1);
     k_at[u] = ((hk << a.page_shift) + (off & in_page) + x / DH16) * DH + x % DH16 * 16;
     v_at[u] = ((hk * DH + x) << a.page_shift) + (off & in_page);
   }
@@ -139,63 +155,67 @@ __global__ __launch_bounds__(64 * RG * KG) __attribute__((amdgpu_waves_per_eu(wa
   auto page_of = [&](int kt, int off, int entry) {
     return (kt >> a.page_shift) + (off >> a.page_shift) < a.max_blocks && kt + (off & ~15) <= hi_g && entry < a.n_pages ? entry : -1;
   };
-  auto pages = [&](int i) { entry = page_entry(key_of(i) + 64 * kg, off); };      // (a step behind the last one begins behind the last row)
-  auto fetch = [&](int i) {      // (what has no page reads the pools' first: no row reads what comes of it)
+  auto entry_of = [&](int i) { return page_entry(key_of(i) + 64 * kg, off); };      // (a step behind the last one begins behind the last row)
+  auto fetch = [&](int i, int entry, Raw& raw) {      // (what has no page reads the pools' first: no row reads what comes of it)
     const int kt = key_of(i) + 64 * kg, far = kt & in_page, judged = page_of(kt, off, entry);
     const uint32_t page = max(judged, 0);
-    there_is = judged >= 0;
+    raw.there = judged >= 0;
     const size_t begin = static_cast<size_t>(page) * page_bytes;
-    k_by = a.k_scale[page * a.Hkv + hk];
-    v_by = a.v_scale[page * a.Hkv + hk];
+    raw.k_by = a.k_scale[page * a.Hkv + hk];
+    raw.v_by = a.v_scale[page * a.Hkv + hk];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      k_raw[u] = *reinterpret_cast<const u32x4*>(a.k_pool + begin + (k_at[u] + far * DH));
-      v_raw[u] = *reinterpret_cast<const u32x4*>(a.v_pool + begin + (v_at[u] + far));
+      raw.k[u] = *reinterpret_cast<const u32x4*>(a.k_pool + begin + (k_at[EVEN ? 0 : u] + (EVEN ? THREADS / 4 / DH16 * DH * u : 0) + far * DH));
+      raw.v[u] = *reinterpret_cast<const u32x4*>(a.v_pool + begin + (v_at[EVEN ? 0 : u] + ((EVEN ? THREADS / 4 * u : 0) << a.page_shift) + far));
     }
   };
-  auto stash = [&](int i, int buf) {
+  auto stash = [&](Raw& raw, int buf) {
     bf16_t* dst = tiles + (buf * KG + kg) * TSZ;
     // Values that are NaN go in as zeros (a weight of zero, of a row that does not read the value, would make NaN of its result), and the
     // rows that do read them are seen to at the end.
     uint32_t nan = 0;
 #pragma unroll
-    for (int u = 0; u < U; ++u) nan |= nan_in(v_raw[u][0]) | nan_in(v_raw[u][1]) | nan_in(v_raw[u][2]) | nan_in(v_raw[u][3]);
+    for (int u = 0; u < U; ++u) nan |= nan_in(raw.v[u][0]) | nan_in(raw.v[u][1]) | nan_in(raw.v[u][2]) | nan_in(raw.v[u][3]);
     if (__builtin_amdgcn_ballot_w64(nan != 0) != 0) {
 #pragma unroll
       for (int u = 0; u < U; ++u)
 #pragma unroll
-        for (int w = 0; w < 4; ++w) v_raw[u][w] &= ~((nan_in(v_raw[u][w]) >> 7) * 0xffu);
-      if (nan != 0 && there_is) *seen = 1;
+        for (int w = 0; w < 4; ++w) raw.v[u][w] &= ~((nan_in(raw.v[u][w]) >> 7) * 0xffu);
+      if (nan != 0 && raw.there) *seen = 1;
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int x = t / 4 + THREADS / 4 * u;
       if (CHUNKS % THREADS == 0 || x < BLOCK_CHUNKS) {
         u32x4* to = reinterpret_cast<u32x4*>(dst + (off + x / DH16) * KROW + x % DH16 * 16);
-        to[0] = widen_scaled(k_raw[u][0], k_raw[u][1], k_by);
-        to[1] = widen_scaled(k_raw[u][2], k_raw[u][3], k_by);
+        to[0] = widen_scaled(raw.k[u][0], raw.k[u][1], raw.k_by);
+        to[1] = widen_scaled(raw.k[u][2], raw.k[u][3], raw.k_by);
         to = reinterpret_cast<u32x4*>(dst + KSZ + x * VROW + off);
-        to[0] = widen_scaled(v_raw[u][0], v_raw[u][2], v_by);
-        to[1] = widen_scaled(v_raw[u][1], v_raw[u][3], v_by);
+        to[0] = widen_scaled(raw.v[u][0], raw.v[u][2], raw.v_by);
+        to[1] = widen_scaled(raw.v[u][1], raw.v[u][3], raw.v_by);
       }
     }
-    if (t < 4) flags[(buf * KG + kg) * 4 + t] = there_is;
+    if (t < 4) flags[(buf * KG + kg) * 4 + t] = raw.there;
   };
 
   if (threadIdx.x == 0) *seen = 0;
   __syncthreads();
-  pages(0);
-  fetch(0);
-  pages(1);
-  stash(0, 0);
-  fetch(1);
-  pages(2);
+  Raw raw;
+  int entry;
+  {      // the first two tiles are asked for at once
+    Raw first;
+    const int entry0 = entry_of(0), entry1 = entry_of(1);
+    entry = entry_of(2);
+    fetch(0, entry0, first);
+    fetch(1, entry1, raw);
+    stash(first, 0);
+  }
   __syncthreads();
   int buf = 0;
   for (int i = 0; i < steps; ++i, buf ^= 1) {
-    if (i + 1 < steps) stash(i + 1, buf ^ 1);
-    if (i + 2 < steps) fetch(i + 2);
-    pages(i + 3);
+    if (i + 1 < steps) stash(raw, buf ^ 1);
+    if (i + 2 < steps) fetch(i + 2, entry, raw);
+    entry = entry_of(i + 3);
 
     const int kw = key_of(i) + 64 * kg;
     // a tile that no row of the wave reads is stepped over

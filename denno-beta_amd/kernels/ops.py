@@ -1011,15 +1011,16 @@ def _single8_shape(n_tiles, n_heads, Hkv, dh, max_context, window, keep_first):
 
 
 def _portions8_shape(n_tiles, n_heads, dh, dtype):
-    """-> (groups of 32 rows, groups of keys) of a workgroup of the portions' kernel.  Where tiles of 128 rows alone give the chip less than a
-    workgroup per CU, halves of them, whose keys two groups share out (a row's time is the keys that its wave walks): 1,001 rows, 25 heads of
-    64, 20.0 us, undivided 26.7.  Up to two and a half per CU the keys only: 2,048 rows 26.1 and 29.3, 2,012 rows of 32 heads of 128
-    behind 2,001 to 8,192 tokens 288 and 301.  Beyond that neither: 4,000 rows behind 1,000 tokens 92 us, with keys shared out 113.  What
-    does not fit the registers so (heads beyond 128; 32-bit ones beyond 96, bfloat16 ones beyond 96 in halves) goes the next best way."""
+    """-> (groups of 32 rows, groups of keys) of a workgroup of the portions' kernel.  Where tiles of 128 rows alone give the chip few
+    workgroups, halves of them, whose keys two groups share out (a row's time is the keys that its wave walks): 1,001 rows, 25 heads of 64, 20.2
+    us, undivided 26.5; 2,048 rows 26.8 and 29.8; 1,001 rows of 16 heads of 96 22.5 and 31.8.  Up to two and a half per CU the keys only: 2,012
+    rows of 32 heads of 128 behind 2,001 to 8,192 tokens 288 and 301.  Beyond that neither: 4,000 rows behind 1,000 tokens 92 us, with keys
+    shared out 117.  What does not fit the registers so (heads beyond 128, 32-bit ones beyond 96, in halves bfloat16 ones beyond 96) goes the
+    next best way."""
     blocks = n_tiles * n_heads
     if dh > (128 if dtype is torch.bfloat16 else 96) or blocks > 640:
         return 4, 1
-    return (2, 2) if blocks <= 256 and dh <= 96 else (4, 2)
+    return (2, 2) if dh <= 96 and blocks <= (256 if dh > 64 else 448) else (4, 2)
 
 
 def _attention8_holds(q, out, block_tables, tiles, n_heads, Hkv, dh):
