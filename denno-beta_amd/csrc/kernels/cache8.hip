@@ -600,10 +600,11 @@ extern "C" int dn_kv_append8(const void* src, int ld, int k_col, int v_col, cons
                     (n_heads == 0 || (whole(src, ld, q_col) && whole(q_out, ldq, 0))) && reinterpret_cast<uintptr_t>(k_pool) % 16 == 0 &&
                     reinterpret_cast<uintptr_t>(v_pool) % 16 == 0;
   if (fast) {
-    // a workgroup for every row as long as that makes no more than 1,024, else for 2, 4, 8, ... rows
+    // A workgroup for every row as long as that makes no more than 1,024, else for 2, 4, 8, ... rows, up to a page's: more would be runs
+    // one after the other (4,096 rows of 25 heads of 64 with 64 rows a workgroup: 126 us).
     const int groups = 2 * ((Hkv + append::HEADS - 1) / append::HEADS), Q = T <= 512 ? 1 : append::UNITS, q_blocks = n_heads > 0 ? (T + Q - 1) / Q : 0;
     int R = 1;
-    while (static_cast<long>((T + R - 1) / R) * groups > 1024 && R < T) R *= 2;
+    while (static_cast<long>((T + R - 1) / R) * groups > 1024 && 2 * R <= page_size) R *= 2;
     const dim3 grid(q_blocks + (T + R - 1) / R * groups);
 #define DN_APPEND(TYPE, HALVES) append::kernel<TYPE, HALVES><<<grid, 64 * append::HEADS, lds_page, stream>>>(a, q_blocks, Q, R)
     if (dtype == DN_F32) {
