@@ -38,6 +38,9 @@ __device__ __forceinline__ u32x4 widen_scaled(uint32_t lo, uint32_t hi, float sc
 // A wait for products that are read behind a branch, which the compiler does not always leave room for: 16 cycles, as a product of 32 x 32 wants at least
 __device__ __forceinline__ void settle(floatx16& a, floatx16& b) { asm volatile("s_nop 15" : "+v"(a), "+v"(b)); }
 
+// the largest scale whose products with all numbers are finite (448 2^119 = 1.75 2^127)
+constexpr float LARGEST = 0x1p119f;
+
 // the upper bit of those of a word's four e4m3 numbers that are NaN (0x7f or 0xff)
 __device__ __forceinline__ uint32_t nan_in(uint32_t w) { return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
 
@@ -176,11 +179,18 @@ __global__ __launch_bounds__(64 * RG * KG) __attribute__((amdgpu_waves_per_eu(wa
     uint32_t nan = 0;
 #pragma unroll
     for (int u = 0; u < U; ++u) nan |= nan_in(raw.v[u][0]) | nan_in(raw.v[u][1]) | nan_in(raw.v[u][2]) | nan_in(raw.v[u][3]);
-    if (__builtin_amdgcn_ballot_w64(nan != 0) != 0) {
+    // So would a value beyond the largest number (256 2^120, which a value above 0.97 of it is rounded to): of a page with a scale so large
+    // numbers go in as at most 240, within the rounding that they have had.  What has no page has no scale either.
+    const float v_by = raw.there ? raw.v_by : 1.0f;
+    if (__builtin_amdgcn_ballot_w64(nan != 0 || v_by > LARGEST) != 0) {
 #pragma unroll
       for (int u = 0; u < U; ++u)
 #pragma unroll
-        for (int w = 0; w < 4; ++w) raw.v[u][w] &= ~((nan_in(raw.v[u][w]) >> 7) * 0xffu);
+        for (int w = 0; w < 4; ++w) {
+          raw.v[u][w] &= ~((nan_in(raw.v[u][w]) >> 7) * 0xffu);
+          const uint32_t high = v_by > LARGEST ? (((raw.v[u][w] & 0x7f7f7f7fu) + 0x08080808u) & 0x80808080u) >> 7 : 0u;      // from 256 on
+          raw.v[u][w] = (raw.v[u][w] & ~(high * 0x7fu)) | high * 0x77u;
+        }
       if (nan != 0 && raw.there) *seen = 1;
     }
 #pragma unroll
@@ -191,8 +201,8 @@ __global__ __launch_bounds__(64 * RG * KG) __attribute__((amdgpu_waves_per_eu(wa
         to[0] = widen_scaled(raw.k[u][0], raw.k[u][1], raw.k_by);
         to[1] = widen_scaled(raw.k[u][2], raw.k[u][3], raw.k_by);
         to = reinterpret_cast<u32x4*>(dst + KSZ + x * VROW + off);
-        to[0] = widen_scaled(raw.v[u][0], raw.v[u][2], raw.v_by);
-        to[1] = widen_scaled(raw.v[u][1], raw.v[u][3], raw.v_by);
+        to[0] = widen_scaled(raw.v[u][0], raw.v[u][2], v_by);
+        to[1] = widen_scaled(raw.v[u][1], raw.v[u][3], v_by);
       }
     }
     if (t < 4) flags[(buf * KG + kg) * 4 + t] = raw.there;

@@ -96,7 +96,8 @@ __global__ __launch_bounds__(WAVES * 64) void kernel(const Args a) {
       for (int c = 0; c < NC; ++c) kr[t][c] = *reinterpret_cast<const u32x4*>(kp + t * 4 * DH + (4 * c + g < DH16 ? c * 64 : -g * 16));
 #pragma unroll
     for (int d = 0; d < DH16; ++d) vr[d] = *reinterpret_cast<const u32x4*>(vp + (static_cast<size_t>(d) * 16 << a.page_shift));
-    const float ks = a.k_scale[vph] * scale2, vs = a.v_scale[vph];
+    const float ks = a.k_scale[vph] * scale2;
+    float vs = a.v_scale[vph];
 
     floatx4 s[4];
 #pragma unroll
@@ -126,7 +127,8 @@ __global__ __launch_bounds__(WAVES * 64) void kernel(const Args a) {
         for (int j = 0; j < 4; ++j) s[t][j] = capped(s[t][j], cap2, to_tanh);
     }
     // a tile at an edge, or with a page that is given back: what the row does not read is -inf, and its values are zeros, whatever
-    // stands there (a weight of zero times NaN would be NaN).  The same for the whole wave.
+    // stands there (a weight of zero times NaN would be NaN), and so is the scale of a block of which it reads nothing.  The same for
+    // the whole wave.
     const bool edge = kt + 63 > pos || kt < lo || __builtin_amdgcn_ballot_w64(v_page < 0) != 0;
     if (edge) {
       uint32_t mask[4] = {0u, 0u, 0u, 0u};
@@ -143,6 +145,7 @@ __global__ __launch_bounds__(WAVES * 64) void kernel(const Args a) {
       for (int d = 0; d < DH16; ++d)
 #pragma unroll
         for (int t = 0; t < 4; ++t) vr[d][t] &= mask[t];
+      vs = (mask[0] | mask[1] | mask[2] | mask[3]) != 0 ? vs : 0.f;
     }
     float top = LOWEST;
 #pragma unroll

@@ -143,6 +143,17 @@ def test_append_far_positions_and_a_factor(turn, mag):
     assert torch.allclose(q_got.cpu(), q_want, atol=0, rtol=2.0 ** -23)
 
 
+@pytest.mark.parametrize("requests", [[(0, 700), (5, 650), (40, 300)], [(0, 2600)]], ids=str)
+def test_append_many_rows(requests):
+    """More rows than there are workgroups for one by one: runs of rows that begin and end inside pages."""
+    for H, hkv, dh, ps, turn, dims in ((33, 33, 16, 16, "none", 0), (2, 9, 16, 64, "halves", 8), (2, 5, 24, 16, "pairs", 24)):
+        _, _, want, got, q_want, q_got = append_both(BF16, H, hkv, dh, ps, requests, turn, dims, seed=len(requests))
+        for name, a, b in zip(("keys", "values", "key scales", "value scales"), got, want):
+            assert same(a, b), name
+        if q_got is not None:
+            assert bool(((q_got.cpu().double() - q_want.double()).abs() <= 2 * (2.0 ** -8 + 2.0 ** -24) * q_want.double().abs() + 1e-300).all())
+
+
 def test_append_leaves_rows_without_a_slot_and_bad_pages():
     """Rows of padding (slot -1) and rows whose page is outside the pools write nothing; their queries are turned like the others'."""
     gen = torch.Generator().manual_seed(2)
@@ -340,6 +351,41 @@ def test_attention_nan_reaches_only_the_rows_that_read_it(dtype, window):
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("dh,bad", [(64, math.nan), (96, math.inf), (20, math.nan)])
+@pytest.mark.parametrize("window", [0, 24])
+def test_attention_scales_of_pages_that_nobody_reads(dtype, dh, bad, window):
+    """Scales that are no numbers, of pages that no row has, the pools' first among them, and of a page behind the window."""
+    for lens, new, single in (([140, 95, 20], [140, 21, 1], False), ([140, 95, 20], [1] * 3, True)):
+        q, pools, bt, tiles, wide = attention_case(lens, new, 4, 2, dh, 16, dtype, seed=15, window=window)
+        k, v = (torch.cat([p.view(torch.uint8)[:1], p.view(torch.uint8)]) for p in pools[:2])
+        k[0] = v[0] = 0x55
+        ks, vs = (torch.cat([torch.full((1, 2), bad), s]) for s in pools[2:])
+        bt = torch.where(bt >= 0, bt + 1, bt)
+        unread = sorted(set(range(k.shape[0])) - set(bt.flatten().tolist()))
+        assert 0 in unread
+        ks[unread] = vs[unread] = bad
+        if window and single:      # the page is still in the table, in the tile of 64 keys that the window begins in
+            bt[0, 4] = unread[-1]
+        check_attention(q, [k.view(FP8), v.view(FP8), ks, vs], bt, tiles, wide, 4, dh ** -0.5, dtype, single=single, longest=140, window=window)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_attention_values_at_the_end_of_the_range(dtype):
+    """A value that has become 2^128 (256 times the scale 2^120) in a portion: the rows before it are as without it."""
+    q, pools, bt, tiles, wide = attention_case([70], [70], 4, 2, 64, 16, dtype, seed=16)
+    q, pools = q.contiguous().to(DEV), [p.to(DEV) for p in pools]
+    bt, tiles, wide = bt.to(DEV), tiles.to(DEV), wide.to(DEV)
+    clean = ops().attention8(q, torch.empty_like(q), *pools, bt, tiles, 4, 0.125, tiles_wide=wide)
+    page = int(bt[0, 3])                                           # positions 48 to 63
+    pools[3][page] = 2.0 ** 120
+    pools[1].view(torch.uint8)[page] = 0x78 | 0x80
+    got = ops().attention8(q, torch.empty_like(q), *pools, bt, tiles, 4, 0.125, tiles_wide=wide)
+    assert torch.equal(got[:48], clean[:48])
+    # one key of such a value, the others' are zeros: weight times 240 2^120, the value's rounding of up to 2^-4 taken off again
+    assert bool((got[48].float() < -2.0 ** 100).all()) and bool(got[48].isfinite().all())
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
 def test_attention_rows_that_read_nothing_and_padding(dtype):
     """A request all of whose pages are given back reads nothing: zeros; rows of padding tiles are left as they were."""
     H, hkv, dh, ps = 4, 2, 64, 16
@@ -489,6 +535,26 @@ def test_two_captured_graphs_of_a_step():
         (x @ x).sum().item()
         for a, b in zip(outs, want):
             assert torch.equal(a, b), turn
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_a_captured_portion(dtype):
+    """Portions whose tiles take more LDS than a workgroup has by itself, captured before they have run otherwise; replays with eager
+    work between them."""
+    H, hkv, dh, ps = 8, 2, 128, 32
+    q, pools, bt, tiles, wide = [x if isinstance(x, list) else x.to(DEV) for x in attention_case([300, 77], [130, 77], H, hkv, dh, ps, dtype, seed=33)]
+    pools = [p.to(DEV) for p in pools]
+    out = torch.zeros(q.shape[0], H * dh, dtype=dtype, device=DEV)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        ops().attention8(q, out, *pools, bt, tiles, H, 0.088, tiles_wide=wide)
+    want = ops().attention8(q, torch.zeros_like(out), *pools, bt, tiles, H, 0.088, tiles_wide=wide)
+    for _ in range(3):
+        out.zero_()
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
+        (pools[2].sum() + 1).item()
 
 
 def test_long_caches_pass_32_bits():
