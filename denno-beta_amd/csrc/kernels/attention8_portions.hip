@@ -461,7 +461,7 @@ extern "C" int dn_attention8_portions(const void* q, int ldq, void* out, int ldo
                                       hipStream_t stream) {
   if (dh < 16 || dh > 256 || dh % 16 != 0 || Hkv < 1 || H % Hkv != 0 || page_size < 16 || (page_size & (page_size - 1)) != 0 || !(scale > 0.f) ||
       n_pages < 1 || max_blocks < 1 || static_cast<size_t>(n_pages) * Hkv >= (1ull << 31) || static_cast<size_t>(Hkv) * dh * page_size >= (1ull << 31) ||
-      window < 0 || keep < 0 || (keep > 0 && window == 0) || !(cap >= 0.f) || ldq % 8 != 0)
+      window < 0 || keep < 0 || (keep > 0 && window == 0) || !(cap >= 0.f && cap < INFINITY) || ldq % 8 != 0)
     return DN_ERR_SHAPE;
   if (dtype != DN_F32 && dtype != DN_BF16) return DN_ERR_DTYPE;
   if (n_tiles == 0) return 0;

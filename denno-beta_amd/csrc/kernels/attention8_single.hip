@@ -283,7 +283,7 @@ extern "C" int dn_attention8_single(const void* q, int ldq, void* out, int ldo, 
                                     int n_splits, int waves, int H, int Hkv, int dh, int page_size, float scale, int window, int keep,
                                     int sink, const float* sink_at, float cap, int dtype, hipStream_t stream) {
   if (dh < 16 || dh > 256 || dh % 16 != 0 || Hkv < 1 || H % Hkv != 0 || page_size < 16 || (page_size & (page_size - 1)) != 0 || window < 0 || keep < 0 ||
-      (keep > 0 && window == 0) || !(cap >= 0.f) || n_splits < 1 || (n_splits > 1 && !part))
+      (keep > 0 && window == 0) || !(cap >= 0.f && cap < INFINITY) || n_splits < 1 || (n_splits > 1 && !part))
     return DN_ERR_SHAPE;
   if (dtype != DN_F32 && dtype != DN_BF16) return DN_ERR_DTYPE;
   if (n_tiles == 0) return 0;

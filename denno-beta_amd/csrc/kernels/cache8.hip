@@ -291,13 +291,16 @@ __device__ __forceinline__ void angles(const Args& a, double* turn, int t0, int 
 }
 
 // A lane's unit u of a row: its two runs of four entries begin at ea and eb.
-template <typename T, bool HALVES>
+// how the first dims of a head are turned
+enum Turn { NOT, PAIRS, HALF };
+
+template <typename T, Turn TURN>
 struct Unit {
   int u, ea, eb, half;
   bool turned;
-  __device__ __forceinline__ Unit(const Args& a, int u_) : u(u_), half(a.dims / 2), turned(u_ < a.dims / 8) {
-    ea = HALVES && turned ? 4 * u : 8 * u;
-    eb = HALVES && turned ? half + 4 * u : 8 * u + 4;
+  __device__ __forceinline__ Unit(const Args& a, int u_) : u(u_), half(a.dims / 2), turned(TURN != NOT && u_ < a.dims / 8) {
+    ea = TURN == HALF && turned ? 4 * u : 8 * u;
+    eb = TURN == HALF && turned ? half + 4 * u : 8 * u + 4;
   }
   __device__ __forceinline__ void load(const T* row, float* v) const { load4(row + ea, v), load4(row + eb, v + 4); }
   // turned as row r's angles say, rounded to 32 bits.  KEYS: so that a second rounding to e4m3 is what rounding the 64-bit number would be,
@@ -311,7 +314,7 @@ struct Unit {
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
       const double* cs = angles + 2 * (r * half + k * (half / 4) + u);
-      const int i = HALVES ? k : 2 * k, j = HALVES ? 4 + k : 2 * k + 1;
+      const int i = TURN == HALF ? k : 2 * k, j = TURN == HALF ? 4 + k : 2 * k + 1;
       const double c = cs[0], s = cs[1], p = v[i], q = v[j];
       w[i] = static_cast<float>(p * c - q * s);
       w[j] = static_cast<float>(q * c + p * s);
@@ -321,7 +324,7 @@ struct Unit {
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         const double* cs = angles + 2 * (r * half + k * (half / 4) + u);
-        const int i = HALVES ? k : 2 * k, j = HALVES ? 4 + k : 2 * k + 1;
+        const int i = TURN == HALF ? k : 2 * k, j = TURN == HALF ? 4 + k : 2 * k + 1;
         const double c = cs[0], s = cs[1], p = v[i], q = v[j];
         w[i] = to_odd(p * c - q * s);
         w[j] = to_odd(q * c + p * s);
@@ -334,10 +337,10 @@ struct Unit {
 constexpr int UNITS = 4, KEY_UNITS = 4;      // units of a lane in flight (keys take more registers)
 
 // rows t0 .. t0 + n (n <= UNITS) of the queries
-template <typename T, bool HALVES>
+template <typename T, Turn TURN>
 __device__ __forceinline__ void turn_queries(const Args& a, double* turn, int t0, int n, int wave, int lane) {
   const int per_row = a.dh / 8, span = 64 / per_row, of = lane / per_row;
-  const Unit<T, HALVES> unit(a, lane % per_row);
+  const Unit<T, TURN> unit(a, lane % per_row);
   const T* x = static_cast<const T*>(a.src) + static_cast<size_t>(t0) * a.ld + a.q_col;
   T* o = static_cast<T*>(a.q_out) + static_cast<size_t>(t0) * a.ldq;
   float v[UNITS][8];
@@ -365,7 +368,7 @@ __device__ __forceinline__ void turn_queries(const Args& a, double* turn, int t0
 }
 
 // The rows t0 .. t0 + n, which stand in one page, of eight key heads (group < ceil(Hkv / 8)) or value heads (the groups behind).
-template <typename T, bool HALVES>
+template <typename T, Turn TURN>
 __device__ __forceinline__ void run_of_rows(const Args& a, double* turn, int* row_in, int group, int t0, int n, int page, int place0, bool odd, int wave,
                                             int lane) {
   const int ps = a.page_size, dh = a.dh, kv_groups = (a.Hkv + HEADS - 1) / HEADS;
@@ -474,7 +477,7 @@ __device__ __forceinline__ void run_of_rows(const Args& a, double* turn, int* ro
 
   // keys: `span` rows at a time
   const int per_row = dh / 8, span = 64 / per_row, of = lane / per_row;
-  const Unit<T, HALVES> unit(a, lane % per_row);
+  const Unit<T, TURN> unit(a, lane % per_row);
   const int end = of < span && head < a.Hkv ? n : 0;      // (a lane without work has no rows)
   const T* x = src + a.k_col + min(head, a.Hkv - 1) * dh;
   float v[KEY_UNITS][8];
@@ -492,7 +495,7 @@ __device__ __forceinline__ void run_of_rows(const Args& a, double* turn, int* ro
   load(0);
   float* scale = a.k_scale + static_cast<size_t>(page) * a.Hkv + head;
   const float was = anew || head >= a.Hkv ? 0.f : *scale;
-  if (a.dims > 0) angles(a, turn, t0, n, wave, lane);
+  if (TURN != NOT) angles(a, turn, t0, n, wave, lane);
   if (head >= a.Hkv) return;      // (no barrier below)
   uint8_t* pool = a.k_pool + (static_cast<size_t>(page) * a.Hkv + head) * ps * dh;
   const bool once = n <= KEY_UNITS * span;
@@ -537,13 +540,15 @@ __device__ __forceinline__ void run_of_rows(const Args& a, double* turn, int* ro
 // The first workgroups take Q rows of queries each.  Of the others, each looks for the runs of rows in one page that begin among its R rows.
 // (A workgroup that finds none costs 2.7 ns of the launch all the same: with one for every row, 2,136 rows of 32 + 8 + 8 heads of
 // 128 took 68 us.)
-template <typename T, bool HALVES>
-__global__ __launch_bounds__(64 * HEADS) __attribute__((amdgpu_waves_per_eu(3))) void kernel(const Args a, int q_blocks, int Q, int R) {
+// Four waves per SIMD where nothing is turned (4,096 rows of 25 heads of 64 21.0 us, with three 26.5; five keep registers in memory), three where
+// the 64-bit numbers want the registers.
+template <typename T, Turn TURN>
+__global__ __launch_bounds__(64 * HEADS) __attribute__((amdgpu_waves_per_eu(TURN == NOT ? 4 : 3))) void kernel(const Args a, int q_blocks, int Q, int R) {
   extern __shared__ double turn[];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64;
-  if (static_cast<int>(blockIdx.x) < q_blocks) {
+  if (TURN != NOT && static_cast<int>(blockIdx.x) < q_blocks) {
     const int t0 = blockIdx.x * Q;
-    turn_queries<T, HALVES>(a, turn, t0, min(Q, a.rows - t0), wave, lane);
+    turn_queries<T, TURN>(a, turn, t0, min(Q, a.rows - t0), wave, lane);
     return;
   }
   int* const row_in = reinterpret_cast<int*>(turn + static_cast<size_t>(a.page_size) * a.dims);
@@ -571,7 +576,7 @@ __global__ __launch_bounds__(64 * HEADS) __attribute__((amdgpu_waves_per_eu(3)))
     for (int r = 63 + lane; r < n; r += 64) odd = odd || a.slot_map[t0 + r] != page * ps + place0 + r;
     odd = __builtin_amdgcn_ballot_w64(odd) != 0;
     // (more rows than places have a slot twice, which is not allowed: those behind are left out, so that what LDS holds suffices)
-    run_of_rows<T, HALVES>(a, turn, row_in, group, t0, min(n, ps), page, place0, odd, wave, lane);
+    run_of_rows<T, TURN>(a, turn, row_in, group, t0, min(n, ps), page, place0, odd, wave, lane);
     t0 += n;
     if (t0 < end) __syncthreads();      // (the next run's angles and places take these ones' room)
   }
@@ -582,7 +587,7 @@ extern "C" int dn_kv_append8(const void* src, int ld, int k_col, int v_col, cons
                              float* k_scale, float* v_scale, int n_pages, const int32_t* positions, const float* freq, int dims,
                              int halves, float mag, int q_col, int n_heads, void* q_out, int ldq, int T, int Hkv, int dh, int page_size,
                              int dtype, hipStream_t stream) {
-  if (dims < 0 || dims % 2 != 0 || dims > dh || dh < 1 || dh > 256 || page_size < 1 || Hkv < 1 || n_heads < 0 || n_pages < 1) return DN_ERR_SHAPE;
+  if (dims < 0 || dims % 2 != 0 || dims > dh || dh < 1 || dh > 256 || page_size < 1 || Hkv < 1 || n_heads < 0 || (n_heads > 0 && dims == 0) || n_pages < 1) return DN_ERR_SHAPE;
   if (dtype != DN_F32 && dtype != DN_BF16) return DN_ERR_DTYPE;
   if (T == 0) return 0;
   int page_shift = 0;
@@ -601,18 +606,20 @@ extern "C" int dn_kv_append8(const void* src, int ld, int k_col, int v_col, cons
                     reinterpret_cast<uintptr_t>(v_pool) % 16 == 0;
   if (fast) {
     // A workgroup for every row as long as that makes no more than 1,024, else for 2, 4, 8, ... rows, up to a page's: more would be runs
-    // one after the other (4,096 rows of 25 heads of 64 with 64 rows a workgroup: 126 us).
+    // one after the other (4,096 rows of 25 heads of 64 with 64 rows a workgroup: 126 us, with 16 21.0).
     const int groups = 2 * ((Hkv + append::HEADS - 1) / append::HEADS), Q = T <= 512 ? 1 : append::UNITS, q_blocks = n_heads > 0 ? (T + Q - 1) / Q : 0;
     int R = 1;
     while (static_cast<long>((T + R - 1) / R) * groups > 1024 && 2 * R <= page_size) R *= 2;
     const dim3 grid(q_blocks + (T + R - 1) / R * groups);
-#define DN_APPEND(TYPE, HALVES) append::kernel<TYPE, HALVES><<<grid, 64 * append::HEADS, lds_page, stream>>>(a, q_blocks, Q, R)
+#define DN_APPEND(TYPE, TURN) append::kernel<TYPE, append::TURN><<<grid, 64 * append::HEADS, lds_page, stream>>>(a, q_blocks, Q, R)
     if (dtype == DN_F32) {
-      if (halves) DN_APPEND(float, true);
-      else DN_APPEND(float, false);
+      if (dims == 0) DN_APPEND(float, NOT);
+      else if (halves) DN_APPEND(float, HALF);
+      else DN_APPEND(float, PAIRS);
     } else {
-      if (halves) DN_APPEND(bf16_t, true);
-      else DN_APPEND(bf16_t, false);
+      if (dims == 0) DN_APPEND(bf16_t, NOT);
+      else if (halves) DN_APPEND(bf16_t, HALF);
+      else DN_APPEND(bf16_t, PAIRS);
     }
 #undef DN_APPEND
   } else {
@@ -705,7 +712,7 @@ extern "C" int dn_attention8(const void* q, int ldq, void* out, int ldo, const v
                              const int32_t* tile_row0, const int32_t* tile_nrows, const int32_t* tile_pos0, int n_tiles, int H, int Hkv,
                              int dh, int page_size, float scale, int window, int keep, int sink, const float* sink_at, float cap,
                              int dtype, hipStream_t stream) {
-  if (dh < 1 || dh > 256 || Hkv < 1 || H % Hkv != 0 || page_size < 1 || window < 0 || keep < 0 || (keep > 0 && window == 0) || !(cap >= 0.f))
+  if (dh < 1 || dh > 256 || Hkv < 1 || H % Hkv != 0 || page_size < 1 || window < 0 || keep < 0 || (keep > 0 && window == 0) || !(cap >= 0.f && cap < INFINITY))
     return DN_ERR_SHAPE;
   if (dtype != DN_F32 && dtype != DN_BF16) return DN_ERR_DTYPE;
   if (n_tiles == 0) return 0;

@@ -897,6 +897,7 @@ def _pools8(k_pool, v_pool, k_scale, v_scale, what):
 
 
 FP8 = torch.float8_e4m3fn
+_INF = float("inf")
 _device_now = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)     # (torch.cuda.current_device asks first whether CUDA is up)
 
 
@@ -1065,7 +1066,7 @@ def attention8(q, out, k_pool, v_pool, k_scale, v_scale, block_tables, tiles, n_
         _attention8_checks(q, out, block_tables, tiles, n_heads, Hkv, dh)
     if sink_at is not None:
         _f32vec(sink_at, "sink", n_heads)
-    _need(window >= 0 and softcap >= 0, "attention8: window or softcap")
+    _need(window >= 0 and 0 <= softcap < _INF, "attention8: window or softcap")
     _need(keep_first >= 0, "attention8: keep_first")
     _one_device("attention8", q, out, k_pool, v_pool, k_scale, v_scale, block_tables, tiles, tiles_wide, sink_at)
     T = q.shape[0]

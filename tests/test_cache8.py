@@ -167,6 +167,8 @@ def test_attention_takes_what_it_documents(monkeypatch):
     ({}, dict(window=-1)),
     ({}, dict(window=4, keep_first=-1)),
     ({}, dict(softcap=-1.0)),
+    ({}, dict(softcap=math.inf)),
+    ({}, dict(softcap=math.nan)),
 ])
 def test_attention_refuses(monkeypatch, change, kw):
     with host_checks_only(monkeypatch), pytest.raises(ops.KernelError):
@@ -200,7 +202,8 @@ def c_append(lib, dims=64, n_heads=0, T=4, hkv=2, dh=64, ps=16, dtype=1, n_pages
 
 def test_append_entry_refuses_before_it_launches(library):
     assert c_append(library, T=0) == 0
-    for kw in (dict(dims=3), dict(dims=66), dict(dims=-2), dict(dh=0, dims=0), dict(dh=257), dict(ps=0), dict(hkv=0), dict(n_heads=-1), dict(n_pages=0)):
+    for kw in (dict(dims=3), dict(dims=66), dict(dims=-2), dict(dh=0, dims=0), dict(dh=257), dict(ps=0), dict(hkv=0), dict(n_heads=-1), dict(n_pages=0),
+               dict(n_heads=1, dims=0)):
         assert c_append(library, **kw) == -2, kw
     assert c_append(library, dtype=2) == -1
     assert c_append(library) > 0      # (no GPU here: the launch itself)
@@ -214,7 +217,7 @@ def c_attend(lib, n_tiles=1, H=4, hkv=2, dh=64, ps=16, window=0, keep=0, cap=0.0
 def test_attention_entry_refuses_before_it_launches(library):
     assert c_attend(library, n_tiles=0) == 0
     for kw in (dict(dh=0), dict(dh=257), dict(hkv=0), dict(hkv=3), dict(ps=0), dict(window=-1), dict(keep=1), dict(keep=-1, window=4),
-               dict(cap=-1.0), dict(cap=math.nan)):
+               dict(cap=-1.0), dict(cap=math.nan), dict(cap=math.inf)):
         assert c_attend(library, **kw) == -2, kw
     assert c_attend(library, dtype=2) == -1
     assert c_attend(library) > 0
