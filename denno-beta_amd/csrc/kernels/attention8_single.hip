@@ -250,25 +250,21 @@ __global__ __launch_bounds__(256) void join_kernel(const Args a, int dh) {
   static_cast<T*>(a.out)[static_cast<size_t>(a.tile_row0[tile]) * a.ldo + head * dh + d] = from_float<T>(l == 0.f ? 0.f : v / l);
 }
 
-template <int DH16, int PARTS, int WAVES>
-static void launch(const Args& a, int n_tiles, hipStream_t stream) {
+template <int DH16, int PARTS>
+static int launch(const Args& a, int n_tiles, hipStream_t stream) {
+  // (heads beyond 128 leave the registers for four waves; up to there eight are faster than four: 16 rows in a window of 4,096 26.8 us and
+  // 29.5, 64 rows over some 700 keys 24.6 and 25.3)
+  constexpr int WAVES = DH16 <= 8 ? 8 : 4;
   const int G = a.H / a.Hkv, blocks = (G + 15) / 16;
   const size_t lds = (2 * WAVES * 16 + static_cast<size_t>(WAVES) * min(G, 16) * (DH16 < 4 ? DH16 * 16 : 64)) * sizeof(float);
   kernel<DH16, PARTS, WAVES><<<dim3(a.n_splits, a.Hkv * blocks, n_tiles), WAVES * 64, lds, stream>>>(a);
-}
-
-template <int DH16, int PARTS>
-static int by_waves(const Args& a, int n_tiles, int waves, hipStream_t stream) {
-  if (waves == 4) launch<DH16, PARTS, 4>(a, n_tiles, stream);
-  else if (waves == 8 && DH16 <= 8) launch<DH16, PARTS, DH16 <= 8 ? 8 : 4>(a, n_tiles, stream);
-  else return DN_ERR_SHAPE;
   return 0;
 }
 
 template <int PARTS>
-static int by_dim(const Args& a, int n_tiles, int dh, int waves, hipStream_t stream) {
+static int by_dim(const Args& a, int n_tiles, int dh, hipStream_t stream) {
   switch (dh / 16) {
-#define DN_DIM(N) case N: return by_waves<N, PARTS>(a, n_tiles, waves, stream);
+#define DN_DIM(N) case N: return launch<N, PARTS>(a, n_tiles, stream);
     DN_DIM(1) DN_DIM(2) DN_DIM(3) DN_DIM(4) DN_DIM(5) DN_DIM(6) DN_DIM(7) DN_DIM(8)
     DN_DIM(9) DN_DIM(10) DN_DIM(11) DN_DIM(12) DN_DIM(13) DN_DIM(14) DN_DIM(15) DN_DIM(16)
 #undef DN_DIM
@@ -280,7 +276,7 @@ static int by_dim(const Args& a, int n_tiles, int dh, int waves, hipStream_t str
 extern "C" int dn_attention8_single(const void* q, int ldq, void* out, int ldo, const void* k_pool, const void* v_pool,
                                     const float* k_scale, const float* v_scale, int n_pages, const int32_t* block_tables, int max_blocks,
                                     const int32_t* tile_seq, const int32_t* tile_row0, const int32_t* tile_pos0, int n_tiles, float* part,
-                                    int n_splits, int waves, int H, int Hkv, int dh, int page_size, float scale, int window, int keep,
+                                    int n_splits, int H, int Hkv, int dh, int page_size, float scale, int window, int keep,
                                     int sink, const float* sink_at, float cap, int dtype, hipStream_t stream) {
   if (dh < 16 || dh > 256 || dh % 16 != 0 || Hkv < 1 || H % Hkv != 0 || page_size < 16 || (page_size & (page_size - 1)) != 0 || window < 0 || keep < 0 ||
       (keep > 0 && window == 0) || !(cap >= 0.f && cap < INFINITY) || n_splits < 1 || (n_splits > 1 && !part))
@@ -290,7 +286,7 @@ extern "C" int dn_attention8_single(const void* q, int ldq, void* out, int ldo, 
   const single8::Args a = {q, out, static_cast<const uint8_t*>(k_pool), static_cast<const uint8_t*>(v_pool), k_scale, v_scale,
                            block_tables, tile_seq, tile_row0, tile_pos0, sink_at, part, ldq, ldo, n_pages, max_blocks, n_splits, H, Hkv,
                            __builtin_ctz(page_size), window, keep, sink, scale, cap};
-  const int rc = dtype == DN_BF16 ? single8::by_dim<1>(a, n_tiles, dh, waves, stream) : single8::by_dim<3>(a, n_tiles, dh, waves, stream);
+  const int rc = dtype == DN_BF16 ? single8::by_dim<1>(a, n_tiles, dh, stream) : single8::by_dim<3>(a, n_tiles, dh, stream);
   if (rc != 0) return rc;
   if (n_splits > 1) {
     if (dtype == DN_BF16) single8::join_kernel<bf16_t><<<dim3(H, n_tiles), 256, 0, stream>>>(a, dh);

@@ -179,7 +179,7 @@ def _declare(name, lib):
         },
         "cache8": {
             "dn_kv_append8": [P, I, I, I, P, P, P, P, P, I, P, P, I, I, F, I, I, P, I, I, I, I, I, I, P],
-            "dn_attention8_single": [P, I, P, I, P, P, P, P, I, P, I, P, P, P, I, P, I, I, I, I, I, I, F, I, I, I, P, F, I, P],
+            "dn_attention8_single": [P, I, P, I, P, P, P, P, I, P, I, P, P, P, I, P, I, I, I, I, I, F, I, I, I, P, F, I, P],
             "dn_attention8_portions": [P, I, P, I, P, P, P, P, I, P, I, P, P, P, P, I, I, I, I, I, I, I, F, I, I, I, P, F, I, P],
             "dn_attention8": [P, I, P, I, P, P, P, P, I, P, I, P, P, P, P, I, I, I, I, I, F, I, I, I, P, F, I, P],
         },
@@ -1000,15 +1000,13 @@ def _append8_checks(src, k_col, v_col, slot_map, positions, freq, q_out, q_col, 
           "kv_append8: q_out is either src's own query columns or memory apart from src")
 
 
-def _single8_shape(n_tiles, n_heads, Hkv, dh, max_context, window, keep_first):
-    """-> (waves of a workgroup, workgroups that a row's keys are shared out to).  One workgroup per CU, as long as every wave has two tiles of
-    64 keys: a row over 131,072 keys with 8 key heads of 128 takes 58 us in 32 x 8 workgroups, 62 in 16 x 8 and 75 in 64 x 8; 518 keys with 25
-    heads of 64 5.0 us undivided and 7.0 in two.  Workgroups of 8 waves (two of them, or heads beyond 128, fill the registers): 16 rows in a window
-    of 4,096 26.8 us, in 4 waves 29.5; 64 rows of GPT-2 XL 24.6 and 25.3."""
+def _single8_splits(n_tiles, n_heads, Hkv, dh, max_context, window, keep_first):
+    """-> how many workgroups a row's keys are shared out to: one per CU, as long as every wave has two tiles of 64 keys.  A row over
+    131,072 keys with 8 key heads of 128 takes 58 us in 32 x 8 workgroups, 62 in 16 x 8 and 75 in 64 x 8; 518 keys with 25 heads of 64 5.0 us
+    undivided and 7.0 in two."""
     reach = max_context if window == 0 else min(max_context, window + keep_first + 128)
     groups = n_tiles * Hkv * -(-(n_heads // Hkv) // 16)
-    waves = 8 if dh <= 128 else 4
-    return waves, max(1, min(-(-reach // 64) // (2 * waves), 256 // groups))
+    return max(1, min(-(-reach // 64) // (16 if dh <= 128 else 8), 256 // groups))      # (workgroups of 8 waves, beyond 128 of 4)
 
 
 def _portions8_shape(n_tiles, n_heads, dh, dtype):
@@ -1081,12 +1079,12 @@ def attention8(q, out, k_pool, v_pool, k_scale, v_scale, block_tables, tiles, n_
         _need(n_tiles == T, "attention8: a step of single rows has a tile for every row")
         _need(max_context <= block_tables.shape[1] * ps, "attention8: max_context exceeds the block tables")
         if aligned:
-            waves, n_splits = _single8_shape(n_tiles, n_heads, Hkv, dh, max_context, window, keep_first)
+            n_splits = _single8_splits(n_tiles, n_heads, Hkv, dh, max_context, window, keep_first)
             part = torch.empty(n_tiles * n_heads * n_splits * (dh + 2), dtype=torch.float32, device=q.device) if n_splits > 1 else None
             _ok(_lib("cache8").dn_attention8_single(
                 q.data_ptr(), ldq, out.data_ptr(), ldo, k_pool.data_ptr(), v_pool.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
                 n_pages, block_tables.data_ptr(), block_tables.shape[1], base, base + 4 * n_tiles, base + 12 * n_tiles, n_tiles, _ptr(part),
-                n_splits, waves, n_heads, Hkv, dh, ps, float(scale), int(window), keep_first, int(sink), _ptr(sink_at), float(softcap),
+                n_splits, n_heads, Hkv, dh, ps, float(scale), int(window), keep_first, int(sink), _ptr(sink_at), float(softcap),
                 _CODE[q.dtype], _stream8()), "attention8 (single rows)")
             return out
     # (the portions' kernel takes the largest score for the largest product: a scale that is not positive goes the plain way)

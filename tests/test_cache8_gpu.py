@@ -409,10 +409,12 @@ def test_attention_rows_that_read_nothing_and_padding(dtype):
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
-@pytest.mark.parametrize("H,hkv,dh", [(4, 2, 16), (2, 2, 64), (4, 1, 80), (3, 3, 128)])
+@pytest.mark.parametrize("H,hkv,dh", [(4, 2, 16), (2, 2, 64), (4, 1, 80), (3, 3, 96), (3, 3, 128)])
 @pytest.mark.parametrize("shape", [(4, 1), (4, 2), (2, 2)], ids=str)
 def test_attention_portions_in_every_shape(monkeypatch, dtype, H, hkv, dh, shape):
     """Every shape of workgroup of the portions' kernel, not only the one that its rule picks for this little work."""
+    if dh > 96 and (shape == (2, 2) or shape == (4, 2) and dtype == F32):
+        pytest.skip("not a shape for these heads")
     o = ops()
     monkeypatch.setattr(o, "_portions8_shape", lambda *a: shape)
     kw = dict(window=150, keep_first=5, sink=True) if dh == 64 else dict(softcap=10.0) if dh == 80 else {}
@@ -422,17 +424,15 @@ def test_attention_portions_in_every_shape(monkeypatch, dtype, H, hkv, dh, shape
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
 @pytest.mark.parametrize("H,hkv,dh", [(4, 2, 16), (40, 2, 64), (3, 3, 128), (2, 1, 208)])
-@pytest.mark.parametrize("waves,splits", [(4, 1), (4, 3), (8, 1), (8, 2), (4, 20)])
-def test_attention_single_rows_in_every_shape(monkeypatch, dtype, H, hkv, dh, waves, splits):
-    """Every number of waves and of workgroups that share a row's keys out, more workgroups than tiles of keys among them."""
-    if waves == 8 and dh > 128:
-        pytest.skip("heads beyond 128 go in workgroups of four waves")
+@pytest.mark.parametrize("splits", [1, 2, 3, 20])
+def test_attention_single_rows_in_every_shape(monkeypatch, dtype, H, hkv, dh, splits):
+    """Every number of workgroups that share a row's keys out, more workgroups than tiles of keys among them."""
     o = ops()
-    monkeypatch.setattr(o, "_single8_shape", lambda *a: (waves, splits))
+    monkeypatch.setattr(o, "_single8_splits", lambda *a: splits)
     kw = dict(window=150, keep_first=5, sink=True) if dh == 64 else {}
     lens = [700, 1, 64, 300]
     case = attention_case(lens, [1] * 4, H, hkv, dh, 16, dtype, seed=dh, window=kw.get("window", 0), keep=kw.get("keep_first", 0))
-    check_attention(*case, H, dh ** -0.5, dtype, single=True, longest=700, what=(waves, splits), **kw)
+    check_attention(*case, H, dh ** -0.5, dtype, single=True, longest=700, what=splits, **kw)
 
 
 def test_attention_shapes_are_refused_by_the_entries():
@@ -440,7 +440,7 @@ def test_attention_shapes_are_refused_by_the_entries():
     q = torch.zeros(1, 256, dtype=BF16, device=DEV)
     p = [t.to(DEV) for t in random_pools(2, 1, 16, 256, torch.Generator().manual_seed(0))]
     bt, tiles = torch.zeros(1, 1, dtype=torch.int32, device=DEV), i32([[0], [0], [1], [0]]).to(DEV)
-    for name, shape, kw in (("_single8_shape", (8, 1), dict(single_rows=True, max_context=1)), ("_portions8_shape", (2, 2), dict(tiles_wide=tiles))):
+    for name, shape, kw in (("_single8_splits", 0, dict(single_rows=True, max_context=1)), ("_portions8_shape", (2, 2), dict(tiles_wide=tiles))):
         real = getattr(o, name)
         setattr(o, name, lambda *a: shape)
         try:
@@ -514,7 +514,7 @@ def test_two_captured_graphs_of_a_step():
         return ops().attention8(turned, torch.empty_like(turned), *pools, bt, tiles, H, dh ** -0.5, single_rows=True, max_context=n)
     states = [state(31, 6000), state(32, 4100)]
     want = [step(s, [p.clone() for p in s[1]]) for s in states]
-    assert ops()._single8_shape(1, H, hkv, dh, 6000, 0, 0)[1] > 1
+    assert ops()._single8_splits(1, H, hkv, dh, 6000, 0, 0) > 1
     side = torch.cuda.Stream()
     side.wait_stream(torch.cuda.current_stream())
     with torch.cuda.stream(side):
