@@ -9,6 +9,7 @@
 namespace append {
 constexpr int ANY_TASKS = 4;     // tasks of a workgroup of the kernel for any size, one a wave
 constexpr int HEADS = 4;         // heads of a workgroup of the other, one a wave
+constexpr int ALL_SIDE_BY_SIDE = 4;      // up to so many rows of a workgroup its runs are all of rows side by side
 constexpr int CHUNK = 16;        // rows whose cos and sin lie in LDS at a time
 constexpr int SCALE_MIN = -117;  // the least exponent of a scale: its smallest number, 2^-9, is then 2^-126, a normal 32-bit one
 
@@ -537,13 +538,17 @@ __device__ __forceinline__ void run_of_rows(const Args& a, double* turn, int* ro
   }
 }
 
-// The first workgroups take Q rows of queries each.  Of the others, each looks for the runs of rows in one page that begin among its R rows.
-// (A workgroup that finds none costs 2.7 ns of the launch all the same: with one for every row, 2,136 rows of 32 + 8 + 8 heads of
-// 128 took 68 us.)
-// Four waves per SIMD where nothing is turned (4,096 rows of 25 heads of 64 21.0 us, with three 26.5; five keep registers in memory), three where
+// The first workgroups take Q rows of queries each.  Of the others, each takes the runs of rows in one page that begin among its R rows side by
+// side.  With more than four of them runs of one row, as decoded tokens are, go to the workgroups in turn instead (block, block + blocks,
+// ...), so that no workgroup has many one after the other: 64 of them in front of 1,984 rows of prompts, 25 heads of 64, 14.6 us, all side by
+// side 26.0 (prompts alone 13.2 and 12.0; 256 single rows, four a workgroup, 14.6 and 13.4).  Runs of pages in turn as well would leave some
+// workgroups two or three of the long ones: 2,799 rows of 32 + 8 + 8 heads of 128 30.4 us for 20.5.
+// (A workgroup that finds none costs 2.7 ns of the launch all the same: with one for every row, 2,136 rows of 32 + 8 + 8 heads of 128 took
+// 68 us.)
+// Four waves per SIMD where nothing is turned (4,096 rows of 25 heads of 64 21.0 us, with three 26.5, before single rows went in turn; five keep registers in memory), three where
 // the 64-bit numbers want the registers.
 template <typename T, Turn TURN>
-__global__ __launch_bounds__(64 * HEADS) __attribute__((amdgpu_waves_per_eu(TURN == NOT ? 4 : 3))) void kernel(const Args a, int q_blocks, int Q, int R) {
+__global__ __launch_bounds__(64 * HEADS) __attribute__((amdgpu_waves_per_eu(TURN == NOT ? 4 : 3))) void kernel(const Args a, int q_blocks, int Q, int R, int blocks) {
   extern __shared__ double turn[];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64;
   if (TURN != NOT && static_cast<int>(blockIdx.x) < q_blocks) {
@@ -551,34 +556,63 @@ __global__ __launch_bounds__(64 * HEADS) __attribute__((amdgpu_waves_per_eu(TURN
     turn_queries<T, TURN>(a, turn, t0, min(Q, a.rows - t0), wave, lane);
     return;
   }
-  int* const row_in = reinterpret_cast<int*>(turn + static_cast<size_t>(a.page_size) * a.dims);
+  int* const row_in = reinterpret_cast<int*>(turn + static_cast<size_t>(min(a.page_size, a.rows)) * a.dims);
   const int groups = 2 * ((a.Hkv + HEADS - 1) / HEADS), group = (blockIdx.x - q_blocks) % groups, block = (blockIdx.x - q_blocks) / groups;
-  const int ps = a.page_size, end = min(a.rows, (block + 1) * R);
-  for (int t0 = block * R; t0 < end;) {
-    // lane i: the slot of row t0 - 1 + i (one load for the row before, the run's length and its places)
-    const int t = t0 - 1 + lane;
-    const int slot = t >= 0 && t < a.rows ? a.slot_map[t] : -1;
-    const int its = a.over_page(slot), its_page = slot < 0 || its >= a.n_pages ? -1 : its;
-    const int page = __builtin_amdgcn_readlane(its_page, 1), place0 = __builtin_amdgcn_readlane(slot - its * ps, 1);
-    if (page < 0) {
-      ++t0;
-      continue;
+  const int ps = a.page_size;
+  auto page_at = [&](int slot) {
+    const int its = a.over_page(slot);
+    return slot < 0 || its >= a.n_pages ? -1 : its;
+  };
+  // slots of the rows from the one before this workgroup's first on, and of the rows that are its own in turn (R <= 32; every wave writes the same)
+  __shared__ int side_by_side[64], in_turn[32];
+  const int first = block * R - 1;
+  uint64_t runs, singles = 0;
+  auto slot_at = [&](int t) { return a.slot_map[min(max(t, 0), a.rows - 1)]; };      // (never a conditional load; what is none is left out behind it)
+  auto is_row = [&](int t) { return t >= 0 && t < a.rows; };
+  int window = slot_at(first + lane);
+  if (R <= ALL_SIDE_BY_SIDE) {
+    window = is_row(first + lane) ? window : -1;
+    const int its = page_at(window), before = __shfl(its, lane - 1);
+    runs = __builtin_amdgcn_ballot_w64(lane >= 1 && lane <= R && its >= 0 && before != its);
+  } else {
+    const int t = block + lane * blocks;
+    int lone = slot_at(t), lone_before = slot_at(t - 1), lone_behind = slot_at(t + 1);
+    window = is_row(first + lane) ? window : -1;
+    lone = lane < R && is_row(t) ? lone : -1;
+    lone_before = t > 0 ? lone_before : -1;
+    lone_behind = t + 1 < a.rows ? lone_behind : -1;
+    if (lane < 32) in_turn[lane] = lone;
+    const int its = page_at(window), before = __shfl(its, lane - 1), behind = __shfl(its, lane + 1), page = page_at(lone);
+    runs = __builtin_amdgcn_ballot_w64(lane >= 1 && lane <= R && its >= 0 && before != its && behind == its);
+    singles = __builtin_amdgcn_ballot_w64(page >= 0 && page_at(lone_before) != page && page_at(lone_behind) != page);
+  }
+  side_by_side[lane] = window;
+  while ((runs | singles) != 0) {
+    int t0, n = 1, slot0;
+    bool odd = false;
+    if (runs != 0) {
+      const int i = __builtin_ctzll(runs);
+      runs &= runs - 1;
+      t0 = first + i;
+      slot0 = __builtin_amdgcn_readlane(window, i);
+      n = __builtin_ctzll(~(__builtin_amdgcn_ballot_w64(page_at(window) == page_at(slot0)) >> i));      // (the bits shifted in are zeros: i >= 1)
+      if (n == 64 - i) n = rows_in_page(a, t0, page_at(slot0), lane);
+      // rows in another order than their places'
+      odd = n > ps - (slot0 - page_at(slot0) * ps) || (lane >= i && lane < i + n && window != slot0 + lane - i);
+      for (int r = 64 - i + lane; r < n; r += 64) odd = odd || a.slot_map[t0 + r] != slot0 + r;
+      odd = __builtin_amdgcn_ballot_w64(odd) != 0;
+    } else {
+      const int i = __builtin_ctzll(singles);
+      singles &= singles - 1;
+      t0 = block + i * blocks;
+      slot0 = __builtin_amdgcn_readfirstlane(in_turn[i]);
     }
-    const uint64_t same = __builtin_amdgcn_ballot_w64(its_page == page);
-    int n = 1 + __builtin_ctzll(~(same >> 2));      // (at most 63: the two bits shifted in are zeros)
-    if (same & 1) {                                 // the row before stands in this page too: this is the rest of another workgroup's run
-      t0 += n;
-      continue;
-    }
-    if (n == 63) n = rows_in_page(a, t0, page, lane);
-    // rows in another order than their places'
-    bool odd = n > ps - place0 || (lane >= 1 && lane <= n && slot != page * ps + place0 + lane - 1);
-    for (int r = 63 + lane; r < n; r += 64) odd = odd || a.slot_map[t0 + r] != page * ps + place0 + r;
-    odd = __builtin_amdgcn_ballot_w64(odd) != 0;
+    const int page = page_at(slot0);
     // (more rows than places have a slot twice, which is not allowed: those behind are left out, so that what LDS holds suffices)
-    run_of_rows<T, TURN>(a, turn, row_in, group, t0, min(n, ps), page, place0, odd, wave, lane);
-    t0 += n;
-    if (t0 < end) __syncthreads();      // (the next run's angles and places take these ones' room)
+    run_of_rows<T, TURN>(a, turn, row_in, group, t0, min(n, ps), page, slot0 - page * ps, odd, wave, lane);
+    if ((runs | singles) == 0) break;
+    __syncthreads();      // (the next run's angles and places take these ones' room)
+    window = side_by_side[lane];      // (so that it takes no register meanwhile)
   }
 }
 }  // namespace append
@@ -595,23 +629,33 @@ extern "C" int dn_kv_append8(const void* src, int ld, int k_col, int v_col, cons
   if ((1 << page_shift) != page_size) page_shift = -1;
   const append::Args a = {src, slot_map, static_cast<uint8_t*>(k_pool), static_cast<uint8_t*>(v_pool), k_scale, v_scale, positions, freq, q_out,
                           ld, k_col, v_col, n_pages, dims, halves, q_col, n_heads, ldq, T, Hkv, dh, page_size, page_shift, mag};
-  // rows of a page in LDS at a time; the kernel for other sizes takes them 16 at a time, whatever the page
-  const size_t lds = static_cast<size_t>(append::CHUNK) * dims * sizeof(double), lds_page = static_cast<size_t>(page_size) * (dims * sizeof(double) + sizeof(int));
+  // a run's rows in LDS at a time, and a page's places; the kernel for other sizes takes rows 16 at a time, whatever the page
+  const size_t lds = static_cast<size_t>(append::CHUNK) * dims * sizeof(double),
+               lds_page = static_cast<size_t>(min(page_size, T)) * dims * sizeof(double) + page_size * sizeof(int);
   const int size = dtype == DN_F32 ? 4 : 2;
   auto whole = [&](const void* p, int stride, int col) {
     return (reinterpret_cast<uintptr_t>(p) + static_cast<size_t>(col) * size) % 16 == 0 && static_cast<size_t>(stride) * size % 16 == 0;
   };
-  const bool fast = dh % 8 == 0 && dims % 8 == 0 && page_size % 16 == 0 && lds_page <= 64 * 1024 && whole(src, ld, k_col) && whole(src, ld, v_col) &&
+  const bool fast = dh % 8 == 0 && dims % 8 == 0 && page_size % 16 == 0 && lds_page <= 128 * 1024 + 4096 && whole(src, ld, k_col) && whole(src, ld, v_col) &&
                     (n_heads == 0 || (whole(src, ld, q_col) && whole(q_out, ldq, 0))) && reinterpret_cast<uintptr_t>(k_pool) % 16 == 0 &&
                     reinterpret_cast<uintptr_t>(v_pool) % 16 == 0;
   if (fast) {
     // A workgroup for every row as long as that makes no more than 1,024, else for 2, 4, 8, ... rows, up to a page's: more would be runs
-    // one after the other (4,096 rows of 25 heads of 64 with 64 rows a workgroup: 126 us, with 16 21.0).
+    // one after the other (4,096 rows of 25 heads of 64 with 64 rows a workgroup: 126 us, with 16 23.4).
     const int groups = 2 * ((Hkv + append::HEADS - 1) / append::HEADS), Q = T <= 512 ? 1 : append::UNITS, q_blocks = n_heads > 0 ? (T + Q - 1) / Q : 0;
     int R = 1;
-    while (static_cast<long>((T + R - 1) / R) * groups > 1024 && 2 * R <= page_size) R *= 2;
-    const dim3 grid(q_blocks + (T + R - 1) / R * groups);
-#define DN_APPEND(TYPE, TURN) append::kernel<TYPE, append::TURN><<<grid, 64 * append::HEADS, lds_page, stream>>>(a, q_blocks, Q, R)
+    while (static_cast<long>((T + R - 1) / R) * groups > 1024 && 2 * R <= min(page_size, 32)) R *= 2;
+    const int blocks = (T + R - 1) / R;
+    const dim3 grid(q_blocks + blocks * groups);
+#define DN_APPEND(TYPE, TURN)                                                                                                          \
+  do {                                                                                                                                 \
+    auto* fn = &append::kernel<TYPE, append::TURN>;                                                                                    \
+    if (lds_page > 60 * 1024) {                                                                                                        \
+      const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(fn), hipFuncAttributeMaxDynamicSharedMemorySize, lds_page); \
+      if (e != hipSuccess) return static_cast<int>(e);                                                                                 \
+    }                                                                                                                                  \
+    fn<<<grid, 64 * append::HEADS, lds_page, stream>>>(a, q_blocks, Q, R, blocks);                                                     \
+  } while (0)
     if (dtype == DN_F32) {
       if (dims == 0) DN_APPEND(float, NOT);
       else if (halves) DN_APPEND(float, HALF);

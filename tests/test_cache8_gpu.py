@@ -84,7 +84,7 @@ def append_both(dtype, H, hkv, dh, ps, requests, turn, dims, mag=1.0, in_place=T
     (4, 4, 64, 16, "none", 0), (8, 2, 128, 16, "pairs", 128), (8, 2, 128, 16, "halves", 128), (5, 5, 80, 32, "halves", 40),
     (6, 3, 48, 8, "pairs", 20), (2, 1, 256, 64, "halves", 256), (3, 3, 15, 16, "pairs", 14), (3, 3, 15, 16, "halves", 6),
     (1, 1, 1, 5, "none", 0), (2, 2, 100, 5, "pairs", 100), (4, 2, 96, 1, "halves", 64), (12, 4, 112, 16, "pairs", 64),
-    (3, 1, 176, 48, "none", 0), (25, 25, 64, 16, "none", 0)])
+    (3, 1, 176, 48, "none", 0), (25, 25, 64, 16, "none", 0), (4, 2, 128, 64, "pairs", 128), (3, 1, 64, 128, "halves", 64)])
 @pytest.mark.parametrize("requests", [DECODE, PORTIONS], ids=["decode", "portions"])
 def test_append(dtype, H, hkv, dh, ps, turn, dims, requests):
     """Numbers and scales are the definition's exactly (both round 64-bit values once); everything outside the rows' pages stays."""
@@ -143,9 +143,11 @@ def test_append_far_positions_and_a_factor(turn, mag):
     assert torch.allclose(q_got.cpu(), q_want, atol=0, rtol=2.0 ** -23)
 
 
-@pytest.mark.parametrize("requests", [[(0, 700), (5, 650), (40, 300)], [(0, 2600)]], ids=str)
+@pytest.mark.parametrize("requests", [[(0, 700), (5, 650), (40, 300)], [(0, 2600)],
+                                      [(17, 1)] * 40 + [(0, 700), (7, 1), (5, 650)] + [(31, 1)] * 30 + [(6, 500), (32, 1)], [(3, 1), (0, 1)] * 300,
+                                      [(15, 2), (14, 3), (16, 1)] * 120], ids=["portions", "a prompt", "mixed", "single rows", "ends of pages"])
 def test_append_many_rows(requests):
-    """More rows than there are workgroups for one by one: runs of rows that begin and end inside pages."""
+    """More rows than there are workgroups for one by one: runs of rows that begin and end inside pages, single ones beside them."""
     for H, hkv, dh, ps, turn, dims in ((33, 33, 16, 16, "none", 0), (2, 9, 16, 64, "halves", 8), (2, 5, 24, 16, "pairs", 24)):
         _, _, want, got, q_want, q_got = append_both(BF16, H, hkv, dh, ps, requests, turn, dims, seed=len(requests))
         for name, a, b in zip(("keys", "values", "key scales", "value scales"), got, want):
