@@ -58,4 +58,42 @@ __device__ __forceinline__ float capped(float s2, float cap2, float to_tanh) {
   return cap2 * fmaf(-2.0f, __builtin_amdgcn_rcpf(e + 1.0f), 1.0f);
 }
 
+// Results of a row's keys that n_splits workgroups shared out, for every row and head: [rows][heads][n_splits][dh + 2], the running maximum
+// (in units of log2(e)), the sum, the weighted values.  A tile's rows are row0 .. row0 + nrows (no nrows: one).
+struct Parts {
+  const float* part;
+  int n_splits;
+  const int32_t *tile_seq, *tile_row0, *tile_nrows;
+  const float* sink_at;
+  int sink, H, dh, ldo;
+};
+
+// the splits' results of a tile's rows and a head, in their order
+template <typename T>
+__global__ __launch_bounds__(256) void join_kernel(const Parts a, T* __restrict__ out) {
+  const int tile = blockIdx.y, head = blockIdx.x;
+  if (a.tile_seq[tile] < 0) return;
+  const int row0 = a.tile_row0[tile], nrows = a.tile_nrows ? a.tile_nrows[tile] : 1;
+  for (int x = blockIdx.z * 256 + threadIdx.x; x < nrows * a.dh; x += 256 * gridDim.z) {
+    const int row = row0 + x / a.dh, d = x % a.dh;
+    const float* part = a.part + (static_cast<size_t>(row) * a.H + head) * a.n_splits * (a.dh + 2);
+    float m = LOWEST, l = 0.f, v = 0.f;
+    for (int s = 0; s < a.n_splits; ++s) m = fmaxf(m, part[static_cast<size_t>(s) * (a.dh + 2)]);
+    for (int s = 0; s < a.n_splits; ++s) {
+      const float* p = part + static_cast<size_t>(s) * (a.dh + 2);
+      const float f = __builtin_amdgcn_exp2f(p[0] - m);
+      l = fmaf(p[1], f, l);
+      v = fmaf(p[2 + d], f, v);
+    }
+    if (a.sink) l += __builtin_amdgcn_exp2f((a.sink_at ? a.sink_at[head] : 0.f) * LOG2E - m);
+    out[static_cast<size_t>(row) * a.ldo + head * a.dh + d] = from_float<T>(l == 0.f ? 0.f : v / l);      // (a row that reads nothing: zeros)
+  }
+}
+
+static inline void join(const Parts& a, void* out, int n_tiles, int dtype, hipStream_t stream) {
+  const dim3 grid(a.H, n_tiles, a.tile_nrows ? 16 : 1);      // (a tile of 128 rows: 8 of them a workgroup)
+  if (dtype == DN_BF16) join_kernel<bf16_t><<<grid, 256, 0, stream>>>(a, static_cast<bf16_t*>(out));
+  else join_kernel<float><<<grid, 256, 0, stream>>>(a, static_cast<float*>(out));
+}
+
 }  // namespace attend8

@@ -22,7 +22,8 @@ struct Args {
   const float *k_scale, *v_scale;
   const int32_t *block_tables, *tile_seq, *tile_row0, *tile_nrows, *tile_pos0;
   const float* sink_at;
-  int ldq, ldo, n_pages, max_blocks, H, Hkv, page_shift, window, keep, sink;      // pages of 1 << page_shift keys
+  float* part;      // attend8::Parts' results, with more than one split
+  int ldq, ldo, n_pages, max_blocks, n_splits, H, Hkv, page_shift, window, keep, sink;      // pages of 1 << page_shift keys
   float scale, cap;
 };
 
@@ -127,6 +128,7 @@ __global__ __launch_bounds__(64 * RG * KG) __attribute__((amdgpu_waves_per_eu(wa
   const int rest = max(lo_g / STEP, kept);
   const int steps = kept + max(0, hi_g / STEP - rest + 1);
   auto key_of = [&](int i) { return STEP * (i < kept ? i : rest + i - kept); };
+  const int share = blockIdx.z, per = (steps + a.n_splits - 1) / a.n_splits, i0 = share * per, i1 = min(steps, i0 + per);      // this workgroup's
 
   // This thread's chunks of its group's tile are all of block t % 4, its 16 keys, so that a thread has one page a tile: chunk x = t / 4 +
   // THREADS / 4 u is, of the keys, 16 dims (x % DH16) of key x / DH16, and of the values dim x.  A tile begins at a multiple of 64, so in
@@ -214,17 +216,17 @@ __global__ __launch_bounds__(64 * RG * KG) __attribute__((amdgpu_waves_per_eu(wa
   int entry;
   {      // the first two tiles are asked for at once
     Raw first;
-    const int entry0 = entry_of(0), entry1 = entry_of(1);
-    entry = entry_of(2);
-    fetch(0, entry0, first);
-    fetch(1, entry1, raw);
+    const int entry0 = entry_of(i0), entry1 = entry_of(i0 + 1);
+    entry = entry_of(i0 + 2);
+    fetch(i0, entry0, first);
+    fetch(i0 + 1, entry1, raw);
     stash(first, 0);
   }
   __syncthreads();
   int buf = 0;
-  for (int i = 0; i < steps; ++i, buf ^= 1) {
-    if (i + 1 < steps) stash(raw, buf ^ 1);
-    if (i + 2 < steps) fetch(i + 2, entry, raw);
+  for (int i = i0; i < i1; ++i, buf ^= 1) {
+    if (i + 1 < i1) stash(raw, buf ^ 1);
+    if (i + 2 < i1) fetch(i + 2, entry, raw);
     entry = entry_of(i + 3);
 
     const int kw = key_of(i) + 64 * kg;
@@ -369,7 +371,17 @@ __global__ __launch_bounds__(64 * RG * KG) __attribute__((amdgpu_waves_per_eu(wa
         for (int i = 0; i < 16; ++i) o[d][i] = o[d][i] * f0 + join[2 + 16 * d + i] * f1;
     }
   }
-  if (row_ok) {
+  float* const part = a.part + ((static_cast<size_t>(row0 + my_row) * a.H + h) * a.n_splits + share) * (DH + 2);      // (of this lane's row)
+  if (row_ok && a.n_splits > 1) {
+    if (g == 0) part[0] = m_run, part[1] = l_run;
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const int dim = 32 * d + 8 * (i / 4) + 4 * g + i % 4;
+        if (dim < DH) part[2 + dim] = o[d][i];
+      }
+  } else if (row_ok) {
     if (a.sink) l_run += __builtin_amdgcn_exp2f((a.sink_at ? a.sink_at[h] : 0.f) * LOG2E - m_run);
     const float inv = l_run == 0.f ? 0.f : 1.0f / l_run;      // (a row that reads nothing: zeros)
     const size_t at = static_cast<size_t>(row0 + my_row) * a.ldo + h * DH;
@@ -394,7 +406,7 @@ __global__ __launch_bounds__(64 * RG * KG) __attribute__((amdgpu_waves_per_eu(wa
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup");
     __builtin_amdgcn_s_waitcnt(0);
     __builtin_amdgcn_wave_barrier();
-    for (int i = 0; i < steps * KG; ++i) {
+    for (int i = i0 * KG; i < i1 * KG; ++i) {
       const int kt = key_of(i / KG) + 64 * (i % KG);
       for (int x = lane; x < DH * 4; x += 64) {
         const int dim = x / 4, first = kt + 16 * (x % 4), page = page_of(kt, 16 * (x % 4), page_entry(kt, 16 * (x % 4)));
@@ -407,7 +419,8 @@ __global__ __launch_bounds__(64 * RG * KG) __attribute__((amdgpu_waves_per_eu(wa
             const int pos = pos0 + r;
             if (key > pos || (key < first_key(pos) && key >= a.keep)) continue;
             const size_t at = static_cast<size_t>(row0 + r) * a.ldo + h * DH + dim;
-            if (PARTS == 1) static_cast<bf16_t*>(a.out)[at] = bf16_t{0x7fc0};
+            if (a.n_splits > 1) a.part[((static_cast<size_t>(row0 + r) * a.H + h) * a.n_splits + share) * (DH + 2) + 2 + dim] = NAN;
+            else if (PARTS == 1) static_cast<bf16_t*>(a.out)[at] = bf16_t{0x7fc0};
             else static_cast<float*>(a.out)[at] = NAN;
           }
         }
@@ -427,7 +440,7 @@ static int launch(const Args& a, int n_tiles, hipStream_t stream) {
     const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(fn), hipFuncAttributeMaxDynamicSharedMemorySize, BYTES);
     if (e != hipSuccess) return static_cast<int>(e);
   }
-  fn<<<dim3(a.H, n_tiles * (4 / RG)), 64 * RG * KG, BYTES, stream>>>(a);
+  fn<<<dim3(a.H, n_tiles * (4 / RG), a.n_splits), 64 * RG * KG, BYTES, stream>>>(a);
   return 0;
 }
 
@@ -458,19 +471,22 @@ static int by_dim(const Args& a, int n_tiles, int dh, int rows, int groups, hipS
 extern "C" int dn_attention8_portions(const void* q, int ldq, void* out, int ldo, const void* k_pool, const void* v_pool,
                                       const float* k_scale, const float* v_scale, int n_pages, const int32_t* block_tables, int max_blocks,
                                       const int32_t* tile_seq, const int32_t* tile_row0, const int32_t* tile_nrows,
-                                      const int32_t* tile_pos0, int n_tiles, int rows, int groups, int H, int Hkv, int dh, int page_size,
-                                      float scale, int window, int keep, int sink, const float* sink_at, float cap, int dtype,
+                                      const int32_t* tile_pos0, int n_tiles, float* part, int n_splits, int rows, int groups, int H,
+                                      int Hkv, int dh, int page_size, float scale, int window, int keep, int sink, const float* sink_at, float cap, int dtype,
                                       hipStream_t stream) {
   if (dh < 16 || dh > 256 || dh % 16 != 0 || Hkv < 1 || H % Hkv != 0 || page_size < 16 || (page_size & (page_size - 1)) != 0 || !(scale > 0.f) ||
       n_pages < 1 || max_blocks < 1 || static_cast<size_t>(n_pages) * Hkv >= (1ull << 31) || static_cast<size_t>(Hkv) * dh * page_size >= (1ull << 31) ||
-      window < 0 || keep < 0 || (keep > 0 && window == 0) || !(cap >= 0.f && cap < INFINITY) || ldq % 8 != 0)
+      window < 0 || keep < 0 || (keep > 0 && window == 0) || !(cap >= 0.f && cap < INFINITY) || ldq % 8 != 0 || n_splits < 1 || (n_splits > 1 && !part))
     return DN_ERR_SHAPE;
   if (dtype != DN_F32 && dtype != DN_BF16) return DN_ERR_DTYPE;
   if (n_tiles == 0) return 0;
   const portions8::Args a = {q, out, static_cast<const uint8_t*>(k_pool), static_cast<const uint8_t*>(v_pool), k_scale, v_scale,
-                             block_tables, tile_seq, tile_row0, tile_nrows, tile_pos0, sink_at, ldq, ldo, n_pages, max_blocks, H, Hkv,
+                             block_tables, tile_seq, tile_row0, tile_nrows, tile_pos0, sink_at, part, ldq, ldo, n_pages, max_blocks, n_splits, H, Hkv,
                              __builtin_ctz(page_size), window, keep, sink, scale, cap};
   const int rc = dtype == DN_BF16 ? portions8::by_dim<1>(a, n_tiles, dh, rows, groups, stream)
                                   : portions8::by_dim<3>(a, n_tiles, dh, rows, groups, stream);
-  return rc != 0 ? rc : dn_launch_status();
+  if (rc != 0) return rc;
+  if (n_splits > 1)
+    attend8::join(attend8::Parts{part, n_splits, tile_seq, tile_row0, tile_nrows, sink_at, sink, H, dh, ldo}, out, n_tiles, dtype, stream);
+  return dn_launch_status();
 }

@@ -23,7 +23,7 @@ struct Args {
   const float *k_scale, *v_scale;
   const int32_t *block_tables, *tile_seq, *tile_row0, *tile_pos0;
   const float* sink_at;
-  float* part;      // [tiles][heads][splits][dh + 2]: maximum, sum, weighted values
+  float* part;      // attend8::Parts' results
   int ldq, ldo, n_pages, max_blocks, n_splits, H, Hkv, page_shift, window, keep, sink;      // pages of 1 << page_shift keys
   float scale, cap;
 };
@@ -216,7 +216,7 @@ __global__ __launch_bounds__(WAVES * 64) void kernel(const Args a) {
       }
       const int head = hk * G + h0 + h;
       if (a.n_splits > 1) {
-        float* part = a.part + ((static_cast<size_t>(tile) * a.H + head) * a.n_splits + sp) * (DH + 2);
+        float* part = a.part + ((static_cast<size_t>(row) * a.H + head) * a.n_splits + sp) * (DH + 2);
         part[2 + d0 * 16 + d] = v;
         if (d0 + d == 0) part[0] = m, part[1] = l;
       } else {
@@ -228,26 +228,6 @@ __global__ __launch_bounds__(WAVES * 64) void kernel(const Args a) {
       }
     }
   }
-}
-
-// the splits' results of a row and head, in their order
-template <typename T>
-__global__ __launch_bounds__(256) void join_kernel(const Args a, int dh) {
-  const int tile = blockIdx.y, head = blockIdx.x;
-  if (a.tile_seq[tile] < 0) return;
-  const float* part = a.part + (static_cast<size_t>(tile) * a.H + head) * a.n_splits * (dh + 2);
-  const int d = threadIdx.x;
-  if (d >= dh) return;
-  float m = LOWEST, l = 0.f, v = 0.f;
-  for (int s = 0; s < a.n_splits; ++s) m = fmaxf(m, part[static_cast<size_t>(s) * (dh + 2)]);
-  for (int s = 0; s < a.n_splits; ++s) {
-    const float* p = part + static_cast<size_t>(s) * (dh + 2);
-    const float f = __builtin_amdgcn_exp2f(p[0] - m);
-    l = fmaf(p[1], f, l);
-    v = fmaf(p[2 + d], f, v);
-  }
-  if (a.sink) l += __builtin_amdgcn_exp2f((a.sink_at ? a.sink_at[head] : 0.f) * LOG2E - m);
-  static_cast<T*>(a.out)[static_cast<size_t>(a.tile_row0[tile]) * a.ldo + head * dh + d] = from_float<T>(l == 0.f ? 0.f : v / l);
 }
 
 template <int DH16, int PARTS>
@@ -288,9 +268,7 @@ extern "C" int dn_attention8_single(const void* q, int ldq, void* out, int ldo, 
                            __builtin_ctz(page_size), window, keep, sink, scale, cap};
   const int rc = dtype == DN_BF16 ? single8::by_dim<1>(a, n_tiles, dh, stream) : single8::by_dim<3>(a, n_tiles, dh, stream);
   if (rc != 0) return rc;
-  if (n_splits > 1) {
-    if (dtype == DN_BF16) single8::join_kernel<bf16_t><<<dim3(H, n_tiles), 256, 0, stream>>>(a, dh);
-    else single8::join_kernel<float><<<dim3(H, n_tiles), 256, 0, stream>>>(a, dh);
-  }
+  if (n_splits > 1)
+    attend8::join(attend8::Parts{part, n_splits, tile_seq, tile_row0, nullptr, sink_at, sink, H, dh, ldo}, out, n_tiles, dtype, stream);
   return dn_launch_status();
 }

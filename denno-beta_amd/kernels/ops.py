@@ -180,7 +180,7 @@ def _declare(name, lib):
         "cache8": {
             "dn_kv_append8": [P, I, I, I, P, P, P, P, P, I, P, P, I, I, F, I, I, P, I, I, I, I, I, I, P],
             "dn_attention8_single": [P, I, P, I, P, P, P, P, I, P, I, P, P, P, I, P, I, I, I, I, I, F, I, I, I, P, F, I, P],
-            "dn_attention8_portions": [P, I, P, I, P, P, P, P, I, P, I, P, P, P, P, I, I, I, I, I, I, I, F, I, I, I, P, F, I, P],
+            "dn_attention8_portions": [P, I, P, I, P, P, P, P, I, P, I, P, P, P, P, I, P, I, I, I, I, I, I, I, F, I, I, I, P, F, I, P],
             "dn_attention8": [P, I, P, I, P, P, P, P, I, P, I, P, P, P, P, I, I, I, I, I, F, I, I, I, P, F, I, P],
         },
         "sampling": {
@@ -1022,6 +1022,15 @@ def _portions8_shape(n_tiles, n_heads, dh, dtype):
     return (2, 2) if dh <= 96 and blocks <= (256 if dh > 64 else 448) else (4, 2)
 
 
+def _portions8_splits(workgroups, groups, max_context, window, keep_first):
+    """-> how many workgroups a tile's keys are shared out to: one per CU, as long as each has four steps (the results that are joined are 32-bit:
+    with more they take longer than the keys).  32 rows of 32 heads of 128 behind 30,000 tokens 85 us in 8 and 536 in one, 64 rows of 25 heads of
+    64 behind 8,000 30.0 in 5 and 98.4, 256 of 32 of 128 behind 8,000 69.4 in 4, 91.4 in 6 and 164 in one; 128 of 12 heads of 64 behind 500
+    stay in one with 13.0 (14.1 in 4)."""
+    reach = max_context if window == 0 else min(max_context, window + keep_first + 256)
+    return max(1, min(reach // (64 * groups) // 4, 256 // workgroups))
+
+
 def _attention8_holds(q, out, block_tables, tiles, n_heads, Hkv, dh):
     """Whether the rows and tables of an ordinary call are right, in one expression (_attention8_checks says what is wrong)."""
     if not (isinstance(q, torch.Tensor) and isinstance(out, torch.Tensor) and isinstance(block_tables, torch.Tensor) and isinstance(tiles, torch.Tensor)
@@ -1051,7 +1060,8 @@ def attention8(q, out, k_pool, v_pool, k_scale, v_scale, block_tables, tiles, n_
     q: [T, >= H*dh], 32-bit or bfloat16, rows contiguous, head h at columns h*dh..; out: [T, H*dh] of q's dtype; query head h reads key head
     h // (H // Hkv).  tiles: int32 [4, n_tiles] = (request, first row, rows <= 16, first position), request < 0: padding;
     tiles_wide: the same rows cut into tiles of up to 128 rows; single_rows: a pure decode step: request s brings row s and is
-    tile s, (s or -1, s, 1, position); max_context: the longest context then.
+    tile s, (s or -1, s, 1, position); max_context: the longest context, a must then; with portions it says how far their keys are worth
+    sharing out (0: not at all).
     window > 0: the row at position p reads the keys from p - window + 1 on, and with keep_first the request's first so many as well;
     sink: True: one more summand exp(0) under the softmax, or 32-bit [H]: exp(sink[h]), which nothing scales; softcap > 0: a scaled score s
     becomes softcap * tanh(s / softcap).
@@ -1093,11 +1103,14 @@ def attention8(q, out, k_pool, v_pool, k_scale, v_scale, block_tables, tiles, n_
         _need(tiles_wide.is_contiguous() and tiles_wide.shape[0] == 4, "attention8: tiles_wide")
         n_wide = tiles_wide.shape[1]
         rows, groups = _portions8_shape(n_wide, n_heads, dh, q.dtype)
+        # (rows of no tile would have room for results as well)
+        n_splits = _portions8_splits(n_wide * n_heads * 4 // rows, groups, max_context, window, keep_first) if 0 < T <= 128 * n_wide else 1
+        part = torch.empty(T * n_heads * n_splits * (dh + 2), dtype=torch.float32, device=q.device) if n_splits > 1 else None
         base = tiles_wide.data_ptr()
         _ok(_lib("cache8").dn_attention8_portions(
             q.data_ptr(), ldq, out.data_ptr(), ldo, k_pool.data_ptr(), v_pool.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
             n_pages, block_tables.data_ptr(), block_tables.shape[1], base, base + 4 * n_wide, base + 8 * n_wide, base + 12 * n_wide, n_wide,
-            rows, groups, n_heads, Hkv, dh, ps, float(scale), int(window), keep_first, int(sink), _ptr(sink_at), float(softcap),
+            _ptr(part), n_splits, rows, groups, n_heads, Hkv, dh, ps, float(scale), int(window), keep_first, int(sink), _ptr(sink_at), float(softcap),
             _CODE[q.dtype], _stream8()), "attention8 (portions)")
         return out
     _ok(_lib("cache8").dn_attention8(

@@ -328,6 +328,9 @@ def test_attention_long_contexts(dtype):
             check_attention(*case, H, dh ** -0.5, dtype, single=True, longest=max(lens), what=("single", lens))
         case = attention_case([1500, 700], [130, 257], H, hkv, dh, ps, dtype, seed=6)
         check_attention(*case, H, dh ** -0.5, dtype, what="portions")
+        case = attention_case([2500, 30], [40, 3], H, hkv, dh, ps, dtype, seed=7)
+        assert ops()._portions8_splits(2 * H * 2, 2, 2500, 0, 0) > 1
+        check_attention(*case, H, dh ** -0.5, dtype, longest=2500, what="few rows")
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
@@ -425,6 +428,39 @@ def test_attention_portions_in_every_shape(monkeypatch, dtype, H, hkv, dh, shape
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("H,hkv,dh", [(4, 2, 16), (2, 2, 64), (4, 1, 80), (3, 3, 128), (2, 1, 208)])
+@pytest.mark.parametrize("splits", [2, 3, 20])
+def test_attention_portions_shared_out(monkeypatch, dtype, H, hkv, dh, splits):
+    """A tile's keys shared out to several workgroups, more workgroups than steps among them."""
+    o = ops()
+    monkeypatch.setattr(o, "_portions8_splits", lambda *a: splits)
+    kw = dict(window=150, keep_first=5, sink=True) if dh == 64 else dict(softcap=10.0, sink=torch.linspace(-2, 3, H)) if dh == 80 else {}
+    case = attention_case([1100, 260, 133, 65], [1, 260, 21, 33], H, hkv, dh, 16, dtype, seed=dh, window=kw.get("window", 0), keep=kw.get("keep_first", 0))
+    check_attention(*case, H, dh ** -0.5, dtype, what=splits, **kw)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("window", [0, 24])
+def test_attention_portions_shared_out_nan_and_padding(monkeypatch, dtype, window):
+    """Keys and values that are NaN in some workgroups' shares reach the rows that read them; a row that reads nothing; rows of no tile."""
+    H, hkv, dh, ps = 4, 2, 64, 16
+    o = ops()
+    monkeypatch.setattr(o, "_portions8_splits", lambda *a: 3)
+    q, pools, bt, tiles, wide = attention_case([600], [140], H, hkv, dh, ps, dtype, seed=8)
+    for pos, which in ((37, 0), (490, 0), (470, 1), (90, 1)):
+        pools[which].view(torch.uint8)[int(bt[0, pos // ps]), which, (pos % ps, 5)[which], (3, pos % ps)[which]] = 0x7f
+    check_attention(q, pools, bt, tiles, wide, H, dh ** -0.5, dtype, window=window)
+    q, pools, bt, tiles, wide = attention_case([400, 50, 600], [20, 1, 30], H, hkv, dh, ps, dtype, seed=10)
+    bt[1] = -1
+    wide[0, 2] = -1
+    got = torch.full((51, H * dh), 9.0, dtype=dtype, device=DEV)
+    want, _, _ = R.attention_exact(q, *pools, bt, tiles, H, dh ** -0.5)
+    o.attention8(q.to(DEV), got, *[p.to(DEV) for p in pools], bt.to(DEV), tiles.to(DEV), H, dh ** -0.5, tiles_wide=wide.to(DEV), max_context=600)
+    assert bool((got[21:] == 9.0).all()) and bool((got[20] == 0).all())
+    assert torch.allclose(got[:20].cpu().double(), want[:20], atol=0.02, rtol=0.02)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
 @pytest.mark.parametrize("H,hkv,dh", [(4, 2, 16), (40, 2, 64), (3, 3, 128), (2, 1, 208)])
 @pytest.mark.parametrize("splits", [1, 2, 3, 20])
 def test_attention_single_rows_in_every_shape(monkeypatch, dtype, H, hkv, dh, splits):
@@ -442,7 +478,8 @@ def test_attention_shapes_are_refused_by_the_entries():
     q = torch.zeros(1, 256, dtype=BF16, device=DEV)
     p = [t.to(DEV) for t in random_pools(2, 1, 16, 256, torch.Generator().manual_seed(0))]
     bt, tiles = torch.zeros(1, 1, dtype=torch.int32, device=DEV), i32([[0], [0], [1], [0]]).to(DEV)
-    for name, shape, kw in (("_single8_splits", 0, dict(single_rows=True, max_context=1)), ("_portions8_shape", (2, 2), dict(tiles_wide=tiles))):
+    for name, shape, kw in (("_single8_splits", 0, dict(single_rows=True, max_context=1)), ("_portions8_shape", (2, 2), dict(tiles_wide=tiles)),
+                            ("_portions8_splits", 0, dict(tiles_wide=tiles))):
         real = getattr(o, name)
         setattr(o, name, lambda *a: shape)
         try:
@@ -540,17 +577,18 @@ def test_two_captured_graphs_of_a_step():
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
-def test_a_captured_portion(dtype):
+@pytest.mark.parametrize("longest", [0, 2300])
+def test_a_captured_portion(dtype, longest):
     """Portions whose tiles take more LDS than a workgroup has by itself, captured before they have run otherwise; replays with eager
-    work between them."""
+    work between them.  With keys shared out the results to be joined are the graph's own memory."""
     H, hkv, dh, ps = 8, 2, 128, 32
-    q, pools, bt, tiles, wide = [x if isinstance(x, list) else x.to(DEV) for x in attention_case([300, 77], [130, 77], H, hkv, dh, ps, dtype, seed=33)]
+    q, pools, bt, tiles, wide = [x if isinstance(x, list) else x.to(DEV) for x in attention_case([2300, 77], [130, 77], H, hkv, dh, ps, dtype, seed=33)]
     pools = [p.to(DEV) for p in pools]
     out = torch.zeros(q.shape[0], H * dh, dtype=dtype, device=DEV)
     g = torch.cuda.CUDAGraph()
     with torch.cuda.graph(g):
-        ops().attention8(q, out, *pools, bt, tiles, H, 0.088, tiles_wide=wide)
-    want = ops().attention8(q, torch.zeros_like(out), *pools, bt, tiles, H, 0.088, tiles_wide=wide)
+        ops().attention8(q, out, *pools, bt, tiles, H, 0.088, tiles_wide=wide, max_context=longest)
+    want = ops().attention8(q, torch.zeros_like(out), *pools, bt, tiles, H, 0.088, tiles_wide=wide, max_context=longest)
     for _ in range(3):
         out.zero_()
         g.replay()
