@@ -460,7 +460,17 @@ __device__ __forceinline__ void run_of_rows(const Args& a, double* turn, int* ro
     for (int i = lane; i < units; i += 64) {
       const int b = i / pairs, d = 2 * (i - b * pairs);
       if (!grown && (b < b0 || b > b1)) continue;
-      if (!once) load_held(d, b), load(d, b);
+      if (!once) {
+        load_held(d, b);
+        if (b >= b0 && b <= b1) {
+          load(d, b);
+        } else {      // a block that no row brings anything to
+#pragma unroll
+          for (int k = 0; k < 16; ++k) y[k][0] = y[k][1] = 0.f;
+#pragma unroll
+          for (int q = 0; q < 4; ++q) mask[q] = 0u;
+        }
+      }
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         u32x4 w;
