@@ -449,8 +449,6 @@ static int by_shape(const Args& a, int n_tiles, int rows, int groups, hipStream_
   if (rows == 4 && groups == 1) return launch<DH16, PARTS, 4, 1>(a, n_tiles, stream);
   if constexpr (DH16 <= (PARTS == 1 ? 8 : 6)) {
     if (rows == 4 && groups == 2) return launch<DH16, PARTS, 4, 2>(a, n_tiles, stream);
-  }
-  if constexpr (DH16 <= 6) {
     if (rows == 2 && groups == 2) return launch<DH16, PARTS, 2, 2>(a, n_tiles, stream);
   }
   return DN_ERR_SHAPE;

@@ -38,7 +38,7 @@ int dn_attention8_single(const void* q, int ldq, void* out, int ldo, const void*
 
 // The same on the matrix cores over tiles of up to 128 rows: head sizes that are multiples of 16, pages of a power of two from 16 keys on, a positive
 // scale, pools and rows 16-byte aligned, ldq a multiple of 8.  A workgroup takes rows (4, or 2) times 32 rows of a tile, its keys shared out to `groups`
-// groups of so many waves: (4, 1), or with heads that leave the registers for it (bfloat16 up to 128, 32-bit up to 96) (4, 2), or up to 96 (2, 2).
+// groups of so many waves: (4, 1), or with heads that leave the registers for it (bfloat16 up to 128, 32-bit up to 96) (4, 2) and (2, 2).
 // n_splits as above; part: H * n_splits * (dh + 2) floats for every row up to the tiles' last.
 int dn_attention8_portions(const void* q, int ldq, void* out, int ldo, const void* k_pool, const void* v_pool, const float* k_scale,
                            const float* v_scale, int n_pages, const int32_t* block_tables, int max_blocks, const int32_t* tile_seq,

@@ -1001,34 +1001,36 @@ def _append8_checks(src, k_col, v_col, slot_map, positions, freq, q_out, q_col, 
 
 
 def _single8_splits(n_tiles, n_heads, Hkv, dh, max_context, window, keep_first):
-    """-> how many workgroups a row's keys are shared out to: one per CU, as long as every wave has two tiles of 64 keys.  A row over
-    131,072 keys with 8 key heads of 128 takes 58 us in 32 x 8 workgroups, 62 in 16 x 8 and 75 in 64 x 8; 518 keys with 25 heads of 64 5.0 us
-    undivided and 7.0 in two."""
+    """-> how many workgroups a row's keys are shared out to: one per CU, as long as every wave has a tile of 64 keys, and none where two tiles a
+    wave are all (the join is a launch of its own).  A row of 32 heads over 8 key heads of 128: 131,072 keys 45.7 us in 32, 53.4 in 16, 50.9
+    in 64; 8,000 keys 10.2 in 16 and 12.5 in 7; 2,000 keys 9.8 in 4 and 14.1 in one; 25 heads of 64 over 1,000 keys 6.5 undivided and 7.4 in two."""
     reach = max_context if window == 0 else min(max_context, window + keep_first + 128)
+    tiles, waves = -(-reach // 64), 8 if dh <= 128 else 4
     groups = n_tiles * Hkv * -(-(n_heads // Hkv) // 16)
-    return max(1, min(-(-reach // 64) // (16 if dh <= 128 else 8), 256 // groups))      # (workgroups of 8 waves, beyond 128 of 4)
+    return max(1, min(-(-tiles // waves), 256 // groups)) if tiles > 2 * waves else 1
 
 
 def _portions8_shape(n_tiles, n_heads, dh, dtype):
     """-> (groups of 32 rows, groups of keys) of a workgroup of the portions' kernel.  Where tiles of 128 rows alone give the chip few
-    workgroups, halves of them, whose keys two groups share out (a row's time is the keys that its wave walks): 1,001 rows, 25 heads of 64, 20.2
-    us, undivided 26.5; 2,048 rows 26.8 and 29.8; 1,001 rows of 16 heads of 96 22.5 and 31.8.  Up to two and a half per CU the keys only: 2,012
-    rows of 32 heads of 128 behind 2,001 to 8,192 tokens 288 and 301.  Beyond that neither: 4,000 rows behind 1,000 tokens 92 us, with keys
-    shared out 117.  What does not fit the registers so (heads beyond 128, 32-bit ones beyond 96, in halves bfloat16 ones beyond 96) goes the
-    next best way."""
+    workgroups, halves of them, whose keys two groups share out (a row's time is the keys that its wave walks), as long as the chip holds them
+    all: 512 rows of 32 heads of 128 16.8 us and 19.6, two times 512 26.8 and 20.6; 1,001 rows of 16 heads of 96 21.6 and 25.7, 853 of 32 heads 35.2 and
+    27.1; heads up to 64, of which a CU holds two, 2,048 rows of 25 26.8 and 29.8.  Up to two and a half per CU the keys only: 2,012
+    rows of 32 heads of 128 behind 2,001 to 8,192 tokens 285 and 290.  Beyond that neither: 4,000 rows behind 1,000 tokens 92 us, with keys
+    shared out 117.  What does not fit the registers so (heads beyond 128, 32-bit ones beyond 96) goes undivided."""
     blocks = n_tiles * n_heads
     if dh > (128 if dtype is torch.bfloat16 else 96) or blocks > 640:
         return 4, 1
-    return (2, 2) if dh <= 96 and blocks <= (256 if dh > 64 else 448) else (4, 2)
+    return (2, 2) if blocks <= (128 if dh > 64 else 448) else (4, 2)
 
 
-def _portions8_splits(workgroups, groups, max_context, window, keep_first):
-    """-> how many workgroups a tile's keys are shared out to: one per CU, as long as each has four steps (the results that are joined are 32-bit:
-    with more they take longer than the keys).  32 rows of 32 heads of 128 behind 30,000 tokens 85 us in 8 and 536 in one, 64 rows of 25 heads of
-    64 behind 8,000 30.0 in 5 and 98.4, 256 of 32 of 128 behind 8,000 69.4 in 4, 91.4 in 6 and 164 in one; 128 of 12 heads of 64 behind 500
-    stay in one with 13.0 (14.1 in 4)."""
+def _portions8_splits(workgroups, groups, dh, max_context, window, keep_first):
+    """-> how many workgroups a tile's keys are shared out to: what the chip holds at a time (of heads up to 64 two per CU), as long as each has so
+    many keys that joining (32-bit results, written and read) takes less than walking them: two steps of heads of 128, four of 64.  32 rows of 32
+    heads of 128 behind 30,000 tokens 80.5 us in 8 and 546 in one; 64 rows of 25 heads of 64 behind 8,000 26.0 in 10, 28.8 in 5, 96.3 in one; 256 rows
+    of 8 heads of 128 behind 3,000 21.9 in 8, 28.4 in 16, 67.6 in one; a prompt of 1,000 rows of 8 heads of 128 25.2 in 2, 25.1 in one, 28.9 in 4; of
+    512 rows of 32 heads 16.6 in one and 36.5 in 2."""
     reach = max_context if window == 0 else min(max_context, window + keep_first + 256)
-    return max(1, min(reach // (64 * groups) // 4, 256 // workgroups))
+    return max(1, min(reach * dh // (64 * groups * 256), (512 if dh <= 64 else 256) // workgroups))
 
 
 def _attention8_holds(q, out, block_tables, tiles, n_heads, Hkv, dh):
@@ -1104,7 +1106,8 @@ def attention8(q, out, k_pool, v_pool, k_scale, v_scale, block_tables, tiles, n_
         n_wide = tiles_wide.shape[1]
         rows, groups = _portions8_shape(n_wide, n_heads, dh, q.dtype)
         # (rows of no tile would have room for results as well)
-        n_splits = _portions8_splits(n_wide * n_heads * 4 // rows, groups, max_context, window, keep_first) if 0 < T <= 128 * n_wide else 1
+        blocks = min(n_wide * 4 // rows, n_wide + T // (32 * rows))      # (of rows; no more than these have any)
+        n_splits = _portions8_splits(blocks * n_heads, groups, dh, max_context, window, keep_first) if 0 < T <= 128 * n_wide else 1
         part = torch.empty(T * n_heads * n_splits * (dh + 2), dtype=torch.float32, device=q.device) if n_splits > 1 else None
         base = tiles_wide.data_ptr()
         _ok(_lib("cache8").dn_attention8_portions(
