@@ -53,8 +53,10 @@ constexpr int waves_per_simd() {      // (with room for one wave only, the compi
 template <int DH16, int PARTS, int RG, int KG>
 __global__ __launch_bounds__(64 * RG * KG) __attribute__((amdgpu_waves_per_eu(waves_per_simd<DH16, PARTS, RG, KG>()))) void kernel(const Args a) {
   constexpr int DH = DH16 * 16, DB = (DH + 31) / 32;
-  constexpr int KROW = DH + 8, VROW = 72;                // elements of a key's row, of a dim's row of 64 keys, 16 bytes of padding each
-  constexpr int KSZ = 64 * KROW, TSZ = KSZ + DH * VROW;  // of a tile's keys, of a tile
+  // elements of a key's row, of a dim's row of 64 keys, 16 bytes of padding each; and 64 bytes more behind every 16 keys, so that the four
+  // blocks of keys that lanes side by side write do not ask for the same banks
+  constexpr int KROW = DH + 8, VROW = 72, BLOCK_PAD = 32;
+  constexpr int KSZ = 64 * KROW + 4 * BLOCK_PAD, TSZ = KSZ + DH * VROW;  // of a tile's keys, of a tile
   constexpr int THREADS = 64 * RG;                       // of a key group
   constexpr int CHUNKS = 64 * DH16;                      // 16-byte chunks of a tile's keys, and of its values
   constexpr int U = (CHUNKS + THREADS - 1) / THREADS;
@@ -199,7 +201,7 @@ __global__ __launch_bounds__(64 * RG * KG) __attribute__((amdgpu_waves_per_eu(wa
     for (int u = 0; u < U; ++u) {
       const int x = t / 4 + THREADS / 4 * u;
       if (CHUNKS % THREADS == 0 || x < BLOCK_CHUNKS) {
-        u32x4* to = reinterpret_cast<u32x4*>(dst + (off + x / DH16) * KROW + x % DH16 * 16);
+        u32x4* to = reinterpret_cast<u32x4*>(dst + (off + x / DH16) * KROW + t % 4 * BLOCK_PAD + x % DH16 * 16);
         to[0] = widen_scaled(raw.k[u][0], raw.k[u][1], raw.k_by);
         to[1] = widen_scaled(raw.k[u][2], raw.k[u][3], raw.k_by);
         to = reinterpret_cast<u32x4*>(dst + KSZ + x * VROW + off);
@@ -225,9 +227,16 @@ __global__ __launch_bounds__(64 * RG * KG) __attribute__((amdgpu_waves_per_eu(wa
   __syncthreads();
   int buf = 0;
   for (int i = i0; i < i1; ++i, buf ^= 1) {
-    if (i + 1 < i1) stash(raw, buf ^ 1);
-    if (i + 2 < i1) fetch(i + 2, entry, raw);
-    entry = entry_of(i + 3);
+    // The next tile on its way to LDS, the one after it to registers: the first key group does this in front of its products, the others behind
+    // theirs, and products go in front of what the other waves of a SIMD do beside them, so that one wave's products run beside another's
+    // other work: 2,012 rows of 32 heads of 128 behind 2,001 to 8,192 tokens 294 -> 275 us, two prompts of 1,024 25.2 -> 24.3 (groups alone 300 and
+    // 24.8, priorities alone 292 and 24.9; with one key group priorities cost, 271 -> 277).
+    auto next = [&]() {
+      if (i + 1 < i1) stash(raw, buf ^ 1);
+      if (i + 2 < i1) fetch(i + 2, entry, raw);
+      entry = entry_of(i + 3);
+    };
+    if (KG == 1 || kg == 0) next();
 
     const int kw = key_of(i) + 64 * kg;
     // a tile that no row of the wave reads is stepped over
@@ -239,7 +248,7 @@ __global__ __launch_bounds__(64 * RG * KG) __attribute__((amdgpu_waves_per_eu(wa
       const u32x4 there4 = *reinterpret_cast<const u32x4*>(flag);      // blocks with a page
       // The operands that LDS gives come four at a time, one such group ahead of the products (a read takes as long as three or four
       // products), the values' first group while the softmax is made.
-      auto key_part = [&](int f) { return *reinterpret_cast<const bf16x8*>(Kb + (32 * (f / DH16) + col) * KROW + f % DH16 * 16 + g * 8); };
+      auto key_part = [&](int f) { return *reinterpret_cast<const bf16x8*>(Kb + f / DH16 * (32 * KROW + 2 * BLOCK_PAD) + col * KROW + col / 16 * BLOCK_PAD + f % DH16 * 16 + g * 8); };
       auto value_part = [&](int f) {      // f: block of 16 keys, then of 32 dims
         return *reinterpret_cast<const bf16x8*>(Vb + min(32 * (f % DB) + col, DH - 1) * VROW + 16 * (f / DB) + 8 * g);
       };
@@ -249,6 +258,7 @@ __global__ __launch_bounds__(64 * RG * KG) __attribute__((amdgpu_waves_per_eu(wa
 #pragma unroll
       for (int j = 0; j < 4; ++j)
         if (j < KF) part[0][j] = key_part(j);
+      if (KG > 1) __builtin_amdgcn_s_setprio(1);
 #pragma unroll
       for (int f = 0; f < KF; f += 4) {
 #pragma unroll
@@ -267,6 +277,7 @@ __global__ __launch_bounds__(64 * RG * KG) __attribute__((amdgpu_waves_per_eu(wa
           }
         __builtin_amdgcn_sched_barrier(0);
       }
+      if (KG > 1) __builtin_amdgcn_s_setprio(0);
       settle(s[0], s[1]);
       const int there = __builtin_amdgcn_readfirstlane(there4[0] | there4[1] << 1 | there4[2] << 2 | there4[3] << 3);
       // an edge: a key that one of the wave's rows does not read.  The same for the whole wave.
@@ -324,6 +335,7 @@ __global__ __launch_bounds__(64 * RG * KG) __attribute__((amdgpu_waves_per_eu(wa
       weigh(0);
       if (DB == 1) weigh(1);
       __builtin_amdgcn_sched_barrier(0);
+      if (KG > 1) __builtin_amdgcn_s_setprio(1);
 #pragma unroll
       for (int f = 0; f < VF; f += 4) {
 #pragma unroll
@@ -339,8 +351,10 @@ __global__ __launch_bounds__(64 * RG * KG) __attribute__((amdgpu_waves_per_eu(wa
           }
         if (f == 0 && DB > 1) weigh(1);
       }
+      if (KG > 1) __builtin_amdgcn_s_setprio(0);
       l_run += (sums[0] + sums[1]) + (sums[2] + sums[3]);
     }
+    if (KG > 1 && kg > 0) next();
     __syncthreads();
   }
   l_run += other_half(l_run);
@@ -432,7 +446,7 @@ __global__ __launch_bounds__(64 * RG * KG) __attribute__((amdgpu_waves_per_eu(wa
 template <int DH16, int PARTS, int RG, int KG>
 static int launch(const Args& a, int n_tiles, hipStream_t stream) {
   constexpr int DH = DH16 * 16, DB = (DH + 31) / 32;
-  constexpr int TILES = 2 * KG * (64 * (DH + 8) + DH * 72) * 2, JOIN = (KG - 1) * 64 * RG * (2 + 16 * DB) * 4;
+  constexpr int TILES = 2 * KG * (64 * (DH + 8) + 128 + DH * 72) * 2, JOIN = (KG - 1) * 64 * RG * (2 + 16 * DB) * 4;
   constexpr int BYTES = (TILES > JOIN ? TILES : JOIN) + 2 * KG * 4 * 4 + 16;
   static_assert(BYTES <= 160 * 1024, "LDS");
   auto* fn = &kernel<DH16, PARTS, RG, KG>;

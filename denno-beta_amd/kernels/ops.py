@@ -1013,12 +1013,12 @@ def _single8_splits(n_tiles, n_heads, Hkv, dh, max_context, window, keep_first):
 def _portions8_shape(n_tiles, n_heads, dh, dtype):
     """-> (groups of 32 rows, groups of keys) of a workgroup of the portions' kernel.  Where tiles of 128 rows alone give the chip few
     workgroups, halves of them, whose keys two groups share out (a row's time is the keys that its wave walks), as long as the chip holds them
-    all: 512 rows of 32 heads of 128 16.8 us and 19.6, two times 512 26.8 and 20.6; 1,001 rows of 16 heads of 96 21.6 and 25.7, 853 of 32 heads 35.2 and
-    27.1; heads up to 64, of which a CU holds two, 2,048 rows of 25 26.8 and 29.8.  Up to two and a half per CU the keys only: 2,012
-    rows of 32 heads of 128 behind 2,001 to 8,192 tokens 285 and 290.  Beyond that neither: 4,000 rows behind 1,000 tokens 92 us, with keys
-    shared out 117.  What does not fit the registers so (heads beyond 128, 32-bit ones beyond 96) goes undivided."""
+    all: 512 rows of 32 heads of 128 16.8 us and 19.6, two times 512 26.8 and 20.6; 1,001 rows of 16 heads of 96 21.6 and 25.7, 853 of 32 heads 25.5 and
+    21.7; heads up to 64, of which a CU holds two, 2,048 rows of 25 24.5 and 25.6.  Up to two per CU the keys only: 1,280 rows of 32 heads of 128 32.8 us and 43.2
+    (behind thousands of tokens both are level: 97.9 and 93.4, 172.7 and 169.7).  Beyond that neither: three prompts of 1,024, 25 heads of 64, 30.2 us, with
+    keys shared out 37.5.  What does not fit the registers so (heads beyond 128, 32-bit ones beyond 96) goes undivided."""
     blocks = n_tiles * n_heads
-    if dh > (128 if dtype is torch.bfloat16 else 96) or blocks > 640:
+    if dh > (128 if dtype is torch.bfloat16 else 96) or blocks > 512:
         return 4, 1
     return (2, 2) if blocks <= (128 if dh > 64 else 448) else (4, 2)
 
