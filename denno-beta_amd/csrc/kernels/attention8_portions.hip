@@ -161,7 +161,7 @@ __global__ __launch_bounds__(64 * RG * KG) __attribute__((amdgpu_waves_per_eu(wa
     v_at[u] = ((hk * DH + x) << a.page_shift) + (off & in_page);
   }
   // The page of the block of 16 keys that key kt + off stands in (off < 64): what the table says is asked for a step before it is
-  // needed (page_entry), and judged when it is (page_of; -1: none, or behind the last row): judged at once, it would be waited for at
+  // needed (page_entry), and looked at when it is (page_of; -1: none, or behind the last row): looked at at once, it would be waited for at
   // once, and with it the keys and values on their way.
   auto page_entry = [&](int kt, int off) { return bt[min((kt >> a.page_shift) + (off >> a.page_shift), a.max_blocks - 1)]; };
   auto page_of = [&](int kt, int off, int entry) {
@@ -169,9 +169,9 @@ __global__ __launch_bounds__(64 * RG * KG) __attribute__((amdgpu_waves_per_eu(wa
   };
   auto entry_of = [&](int i) { return page_entry(key_of(i) + 64 * kg, off); };      // (a step behind the last one begins behind the last row)
   auto fetch = [&](int i, int entry, Raw& raw) {      // (what has no page reads the pools' first: no row reads what comes of it)
-    const int kt = key_of(i) + 64 * kg, far = kt & in_page, judged = page_of(kt, off, entry);
-    const uint32_t page = max(judged, 0);
-    raw.there = judged >= 0;
+    const int kt = key_of(i) + 64 * kg, far = kt & in_page, found = page_of(kt, off, entry);
+    const uint32_t page = max(found, 0);
+    raw.there = found >= 0;
     const size_t begin = static_cast<size_t>(page) * page_bytes;
     raw.k_by = a.k_scale[page * a.Hkv + hk];
     raw.v_by = a.v_scale[page * a.Hkv + hk];

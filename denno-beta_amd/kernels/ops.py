@@ -876,14 +876,6 @@ def attention(q, out, k_pool, v_pool, block_tables, tiles, n_heads, scale, windo
 
 def _pools8(k_pool, v_pool, k_scale, v_scale, what):
     """The cache in 8 bits: -> (n_pages, Hkv, page_size, dh)."""
-    # (one expression for what holds in front of every layer's launch; where it does not, the checks below say what is wrong)
-    if (isinstance(k_pool, torch.Tensor) and k_pool.dtype is FP8 and k_pool.is_cuda and k_pool.dim() == 4 and isinstance(v_pool, torch.Tensor)
-            and v_pool.dtype is FP8 and v_pool.is_cuda and isinstance(k_scale, torch.Tensor) and isinstance(v_scale, torch.Tensor)
-            and k_scale.dtype is v_scale.dtype is torch.float32 and k_scale.is_cuda and v_scale.is_cuda):
-        n_pages, Hkv, ps, dh = shape = k_pool.shape
-        if (0 not in shape and dh <= 256 and v_pool.shape == (n_pages, Hkv, dh, ps) and k_scale.shape == v_scale.shape == (n_pages, Hkv)
-                and k_pool.is_contiguous() and v_pool.is_contiguous() and k_scale.is_contiguous() and v_scale.is_contiguous()):
-            return shape
     _dev(k_pool, "k_pool", (FP8,), 4), _dev(v_pool, "v_pool", (FP8,), 4)
     _dev(k_scale, "k_scale", (torch.float32,), 2), _dev(v_scale, "v_scale", (torch.float32,), 2)
     n_pages, Hkv, ps, dh = k_pool.shape
@@ -897,13 +889,25 @@ def _pools8(k_pool, v_pool, k_scale, v_scale, what):
 
 
 FP8 = torch.float8_e4m3fn
-_INF = float("inf")
+_F32_TYPE, _I32_TYPE, _INF = torch.float32, torch.int32, float("inf")
 _device_now = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)     # (torch.cuda.current_device asks first whether CUDA is up)
+_NOT_TENSORS = (AttributeError, TypeError, ValueError, IndexError)      # what a wrong argument makes of the expressions below
+
+# These two functions' calls stand in front of every layer's launch, and half of a call's time was their checks.  So each looks first, in one
+# expression (_append8_holds, _attention8_holds: no check twice, none that another implies: 8.3 -> 7.1 us of Python a call), whether all is as in
+# an ordinary call; where it is not, the checks one by one say what is wrong, or let pass what is right all the same.
 
 
-def _stream8():
-    """_stream(), for tensors that _one_device has seen on the current device."""
-    return _raw_stream(_device_now()) if _raw_stream is not None else _stream()
+def _pools8_hold(device, n_pages, Hkv, ps, dh, k_pool, v_pool, k_scale, v_scale):
+    return (k_pool.dtype is v_pool.dtype is FP8 and k_scale.dtype is v_scale.dtype is _F32_TYPE and n_pages > 0 and Hkv > 0 and ps > 0 and 0 < dh <= 256
+            and device == k_pool.get_device() == v_pool.get_device() == k_scale.get_device() == v_scale.get_device()
+            and v_pool.shape == (n_pages, Hkv, dh, ps) and k_scale.shape == v_scale.shape == (n_pages, Hkv)
+            and k_pool.is_contiguous() and v_pool.is_contiguous() and k_scale.is_contiguous() and v_scale.is_contiguous())
+
+
+def _stream8(device):
+    """The stream of tensors that have been seen on the current device, `device`."""
+    return _raw_stream(device) if _raw_stream is not None else _stream()
 
 
 def _one_device(what, *tensors):
@@ -931,10 +935,12 @@ def kv_append8(src, k_col, v_col, slot_map, k_pool, v_pool, k_scale, v_scale, po
     freq: 32-bit [dims / 2]: the first `dims` entries of every key are turned in pairs, entries 2i and 2i + 1, or with halves i and
     i + dims / 2, by the angle positions[t] * freq[i] (cos and sin times mag; in 64 bits until the one rounding).  q_out [T, n_heads * dh] of src's
     dtype: the queries at columns q_col.. of src, turned the same way (it may be those columns themselves)."""
-    n_pages, Hkv, ps, dh = _pools8(k_pool, v_pool, k_scale, v_scale, "kv_append8")
-    if not _append8_holds(src, k_col, v_col, slot_map, positions, freq, q_out, q_col, n_heads, Hkv, dh):
-        _append8_checks(src, k_col, v_col, slot_map, positions, freq, q_out, q_col, n_heads, Hkv, dh)
-    _one_device("kv_append8", src, slot_map, k_pool, v_pool, k_scale, v_scale, positions, freq, q_out)
+    shape = _append8_holds(src, k_col, v_col, slot_map, k_pool, v_pool, k_scale, v_scale, positions, freq, q_out, q_col, n_heads)
+    if shape is None:
+        shape = _pools8(k_pool, v_pool, k_scale, v_scale, "kv_append8")
+        _append8_checks(src, k_col, v_col, slot_map, positions, freq, q_out, q_col, n_heads, shape[1], shape[3])
+        _one_device("kv_append8", src, slot_map, k_pool, v_pool, k_scale, v_scale, positions, freq, q_out)
+    n_pages, Hkv, ps, dh = shape
     T = src.shape[0]
     if T == 0:
         return
@@ -943,34 +949,36 @@ def kv_append8(src, k_col, v_col, slot_map, k_pool, v_pool, k_scale, v_scale, po
     _ok(_lib("cache8").dn_kv_append8(src.data_ptr(), ld, k_col, v_col, slot_map.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(),
                                      k_scale.data_ptr(), v_scale.data_ptr(), n_pages, positions.data_ptr() if dims else None,
                                      freq.data_ptr() if dims else None, dims, 1 if halves else 0, float(mag), q_col, n_heads,
-                                     q_out.data_ptr() if ldq else None, ldq, T, Hkv, dh, ps, _CODE[src.dtype], _stream8()), "kv_append8")
+                                     q_out.data_ptr() if ldq else None, ldq, T, Hkv, dh, ps, _CODE[src.dtype], _stream8(src.get_device())), "kv_append8")
 
 
-def _append8_holds(src, k_col, v_col, slot_map, positions, freq, q_out, q_col, n_heads, Hkv, dh):
-    """Whether the rows of an ordinary call are right, in one expression (_append8_checks says what is wrong): queries in front of the
-    keys, and turned in memory apart from src or where they stand."""
-    if not (isinstance(src, torch.Tensor) and isinstance(slot_map, torch.Tensor) and src.is_cuda and slot_map.is_cuda and src.dim() == 2):
-        return False
-    T, width = src.shape
-    w, stride = Hkv * dh, src.stride()
-    if not (src.dtype in _CODE and stride[1] == 1 and stride[0] >= width and slot_map.dtype is torch.int32 and slot_map.shape == (T,)
-            and slot_map.is_contiguous() and 0 <= k_col <= width - w and 0 <= v_col <= width - w):
-        return False
-    if freq is None:
-        return q_out is None and n_heads == 0
-    if not (isinstance(freq, torch.Tensor) and isinstance(positions, torch.Tensor) and freq.dtype is torch.float32 and freq.is_cuda and positions.is_cuda
-            and positions.dtype is torch.int32 and positions.shape == (T,) and 2 <= 2 * freq.numel() <= dh and freq.is_contiguous()
-            and positions.is_contiguous()):
-        return False
-    if q_out is None:
-        return n_heads == 0
-    qw = n_heads * dh
-    if not (isinstance(q_out, torch.Tensor) and q_out.dtype is src.dtype and n_heads >= 1 and q_out.shape == (T, qw) and 0 <= q_col
-            and q_col + qw <= k_col <= v_col):
-        return False
-    size, at, own, sq = src.element_size(), q_out.data_ptr(), src.data_ptr(), q_out.stride()
-    return sq[1] == 1 and sq[0] >= qw and T > 1 and (at == own + q_col * size and sq[0] == stride[0] or at >= own + ((T - 1) * stride[0] + width) * size
-                                                    or at + ((T - 1) * sq[0] + qw) * size <= own)
+def _append8_holds(src, k_col, v_col, slot_map, k_pool, v_pool, k_scale, v_scale, positions, freq, q_out, q_col, n_heads):
+    """The pools' shape if an ordinary call's arguments are right (queries in front of the keys, and turned in memory apart from src or where
+    they stand), else None."""
+    try:
+        n_pages, Hkv, ps, dh = shape = k_pool.shape
+        T, width = src.shape
+        w, (ld, one), device = Hkv * dh, src.stride(), src.get_device()
+        if not (src.dtype in _CODE and one == 1 and ld >= width and slot_map.dtype is _I32_TYPE and slot_map.shape == (T,) and slot_map.is_contiguous()
+                and 0 <= k_col <= width - w and 0 <= v_col <= width - w and device == slot_map.get_device() and device >= 0 and device == _device_now()
+                and _pools8_hold(device, n_pages, Hkv, ps, dh, k_pool, v_pool, k_scale, v_scale)):
+            return None
+        if freq is None:
+            return shape if q_out is None and n_heads == 0 else None
+        if not (freq.dtype is _F32_TYPE and positions.dtype is _I32_TYPE and positions.shape == (T,) and 2 <= 2 * freq.numel() <= dh
+                and freq.is_contiguous() and positions.is_contiguous() and device == freq.get_device() == positions.get_device()):
+            return None
+        if q_out is None:
+            return shape if n_heads == 0 else None
+        qw, (ldq, one) = n_heads * dh, q_out.stride()
+        if not (T > 1 and n_heads >= 1 and q_out.dtype is src.dtype and q_out.shape == (T, qw) and one == 1 and ldq >= qw and 0 <= q_col
+                and q_col + qw <= k_col <= v_col and device == q_out.get_device()):
+            return None
+        size, at, own = src.element_size(), q_out.data_ptr(), src.data_ptr()
+        apart = at >= own + ((T - 1) * ld + width) * size or at + ((T - 1) * ldq + qw) * size <= own
+        return shape if apart or (at == own + q_col * size and ldq == ld) else None
+    except _NOT_TENSORS:
+        return None
 
 
 def _append8_checks(src, k_col, v_col, slot_map, positions, freq, q_out, q_col, n_heads, Hkv, dh):
@@ -1033,16 +1041,23 @@ def _portions8_splits(workgroups, groups, dh, max_context, window, keep_first):
     return max(1, min(reach * dh // (64 * groups * 256), (512 if dh <= 64 else 256) // workgroups))
 
 
-def _attention8_holds(q, out, block_tables, tiles, n_heads, Hkv, dh):
-    """Whether the rows and tables of an ordinary call are right, in one expression (_attention8_checks says what is wrong)."""
-    if not (isinstance(q, torch.Tensor) and isinstance(out, torch.Tensor) and isinstance(block_tables, torch.Tensor) and isinstance(tiles, torch.Tensor)
-            and q.is_cuda and out.is_cuda and block_tables.is_cuda and tiles.is_cuda and q.dim() == 2 and out.dim() == 2 and n_heads > 0):
-        return False
-    T, width = q.shape
-    w, sq, so = n_heads * dh, q.stride(), out.stride()
-    return (q.dtype in _CODE and out.dtype is q.dtype and block_tables.dtype is tiles.dtype is torch.int32 and n_heads % Hkv == 0 and width >= w
-            and out.shape == (T, w) and sq[1] == so[1] == 1 and sq[0] >= width and so[0] >= w and block_tables.dim() == 2 and tiles.dim() == 2
-            and tiles.shape[0] == 4 and block_tables.is_contiguous() and tiles.is_contiguous())
+def _attention8_holds(q, out, k_pool, v_pool, k_scale, v_scale, block_tables, tiles, n_heads):
+    """The pools' shape if an ordinary call's rows and tables are right, else None."""
+    try:
+        n_pages, Hkv, ps, dh = shape = k_pool.shape
+        T, width = q.shape
+        w, (ldq, one), (ldo, two), device, dtype = n_heads * dh, q.stride(), out.stride(), q.get_device(), q.dtype
+        four, _ = tiles.shape
+        _, _ = block_tables.shape
+        if (n_heads > 0 and n_heads % Hkv == 0 and dtype in _CODE and out.dtype is dtype and block_tables.dtype is tiles.dtype is _I32_TYPE
+                and width >= w and out.shape == (T, w) and one == two == 1 and ldq >= width and ldo >= w and four == 4
+                and block_tables.is_contiguous() and tiles.is_contiguous()
+                and device == out.get_device() == block_tables.get_device() == tiles.get_device() and device >= 0 and device == _device_now()
+                and _pools8_hold(device, n_pages, Hkv, ps, dh, k_pool, v_pool, k_scale, v_scale)):
+            return shape
+    except (ZeroDivisionError, *_NOT_TENSORS):
+        pass
+    return None
 
 
 def _attention8_checks(q, out, block_tables, tiles, n_heads, Hkv, dh):
@@ -1069,19 +1084,22 @@ def attention8(q, out, k_pool, v_pool, k_scale, v_scale, block_tables, tiles, n_
     becomes softcap * tanh(s / softcap).
     Rows of padding tiles are left as they were.  What stands in places that a row does not read does not reach it, NaN included;
     a page that is given back (a negative entry) is not read; a row that reads nothing becomes zeros."""
-    n_pages, Hkv, ps, dh = _pools8(k_pool, v_pool, k_scale, v_scale, "attention8")
+    shape = _attention8_holds(q, out, k_pool, v_pool, k_scale, v_scale, block_tables, tiles, n_heads)
+    if shape is None:
+        shape = _pools8(k_pool, v_pool, k_scale, v_scale, "attention8")
+        _attention8_checks(q, out, block_tables, tiles, n_heads, shape[1], shape[3])
+        _one_device("attention8", q, out, k_pool, v_pool, k_scale, v_scale, block_tables, tiles)
+    n_pages, Hkv, ps, dh = shape
     sink_at, sink = (sink, True) if isinstance(sink, torch.Tensor) else (None, bool(sink))
     keep_first = int(keep_first) if window > 0 else 0      # (without a window every key is read anyway)
-    if not _attention8_holds(q, out, block_tables, tiles, n_heads, Hkv, dh):
-        _attention8_checks(q, out, block_tables, tiles, n_heads, Hkv, dh)
     if sink_at is not None:
         _f32vec(sink_at, "sink", n_heads)
-    _need(window >= 0 and 0 <= softcap < _INF, "attention8: window or softcap")
-    _need(keep_first >= 0, "attention8: keep_first")
-    _one_device("attention8", q, out, k_pool, v_pool, k_scale, v_scale, block_tables, tiles, tiles_wide, sink_at)
+        _one_device("attention8", sink_at)
+    if not (window >= 0 and 0 <= softcap < _INF and keep_first >= 0):
+        raise KernelError("attention8: window, keep_first or softcap")
     T = q.shape[0]
     ldq, ldo = (q.stride(0), out.stride(0)) if T > 1 else (q.shape[1], out.shape[1])
-    n_tiles = tiles.shape[1]
+    n_tiles, max_blocks = tiles.shape[1], block_tables.shape[1]
     if T == 0 or n_tiles == 0:
         return out
     base = tiles.data_ptr()
@@ -1089,19 +1107,20 @@ def attention8(q, out, k_pool, v_pool, k_scale, v_scale, block_tables, tiles, n_
     aligned = (dh % 16 == 0 and ps >= 16 and ps & (ps - 1) == 0 and k_pool.data_ptr() % 16 == 0 and v_pool.data_ptr() % 16 == 0)
     if single_rows and max_context > 0:
         _need(n_tiles == T, "attention8: a step of single rows has a tile for every row")
-        _need(max_context <= block_tables.shape[1] * ps, "attention8: max_context exceeds the block tables")
+        _need(max_context <= max_blocks * ps, "attention8: max_context exceeds the block tables")
         if aligned:
             n_splits = _single8_splits(n_tiles, n_heads, Hkv, dh, max_context, window, keep_first)
             part = torch.empty(n_tiles * n_heads * n_splits * (dh + 2), dtype=torch.float32, device=q.device) if n_splits > 1 else None
             _ok(_lib("cache8").dn_attention8_single(
                 q.data_ptr(), ldq, out.data_ptr(), ldo, k_pool.data_ptr(), v_pool.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
-                n_pages, block_tables.data_ptr(), block_tables.shape[1], base, base + 4 * n_tiles, base + 12 * n_tiles, n_tiles, _ptr(part),
+                n_pages, block_tables.data_ptr(), max_blocks, base, base + 4 * n_tiles, base + 12 * n_tiles, n_tiles, _ptr(part),
                 n_splits, n_heads, Hkv, dh, ps, float(scale), int(window), keep_first, int(sink), _ptr(sink_at), float(softcap),
-                _CODE[q.dtype], _stream8()), "attention8 (single rows)")
+                _CODE[q.dtype], _stream8(q.get_device())), "attention8 (single rows)")
             return out
     # (the portions' kernel takes the largest score for the largest product: a scale that is not positive goes the plain way)
     if aligned and tiles_wide is not None and scale > 0 and ldq % 8 == 0 and q.data_ptr() % 16 == 0:
         _dev(tiles_wide, "tiles_wide", _I32, 2)
+        _one_device("attention8", tiles_wide)
         _need(tiles_wide.is_contiguous() and tiles_wide.shape[0] == 4, "attention8: tiles_wide")
         n_wide = tiles_wide.shape[1]
         rows, groups = _portions8_shape(n_wide, n_heads, dh, q.dtype)
@@ -1112,14 +1131,14 @@ def attention8(q, out, k_pool, v_pool, k_scale, v_scale, block_tables, tiles, n_
         base = tiles_wide.data_ptr()
         _ok(_lib("cache8").dn_attention8_portions(
             q.data_ptr(), ldq, out.data_ptr(), ldo, k_pool.data_ptr(), v_pool.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
-            n_pages, block_tables.data_ptr(), block_tables.shape[1], base, base + 4 * n_wide, base + 8 * n_wide, base + 12 * n_wide, n_wide,
+            n_pages, block_tables.data_ptr(), max_blocks, base, base + 4 * n_wide, base + 8 * n_wide, base + 12 * n_wide, n_wide,
             _ptr(part), n_splits, rows, groups, n_heads, Hkv, dh, ps, float(scale), int(window), keep_first, int(sink), _ptr(sink_at), float(softcap),
-            _CODE[q.dtype], _stream8()), "attention8 (portions)")
+            _CODE[q.dtype], _stream8(q.get_device())), "attention8 (portions)")
         return out
     _ok(_lib("cache8").dn_attention8(
         q.data_ptr(), ldq, out.data_ptr(), ldo, k_pool.data_ptr(), v_pool.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), n_pages,
-        block_tables.data_ptr(), block_tables.shape[1], base, base + 4 * n_tiles, base + 8 * n_tiles, base + 12 * n_tiles, n_tiles, n_heads,
-        Hkv, dh, ps, float(scale), int(window), keep_first, int(sink), _ptr(sink_at), float(softcap), _CODE[q.dtype], _stream8()), "attention8")
+        block_tables.data_ptr(), max_blocks, base, base + 4 * n_tiles, base + 8 * n_tiles, base + 12 * n_tiles, n_tiles, n_heads,
+        Hkv, dh, ps, float(scale), int(window), keep_first, int(sink), _ptr(sink_at), float(softcap), _CODE[q.dtype], _stream8(q.get_device())), "attention8")
     return out
 
 

@@ -1,5 +1,5 @@
 """The cache in 8 bits without a GPU: what its functions refuse, what its C entries refuse before they launch anything, and the
-definitions by which the GPU tests judge."""
+definitions that the GPU tests compare with."""
 import contextlib
 import ctypes
 import math
