@@ -971,12 +971,12 @@ def _append8_holds(src, k_col, v_col, slot_map, k_pool, v_pool, k_scale, v_scale
         if q_out is None:
             return shape if n_heads == 0 else None
         qw, (ldq, one) = n_heads * dh, q_out.stride()
-        if not (T > 1 and n_heads >= 1 and q_out.dtype is src.dtype and q_out.shape == (T, qw) and one == 1 and ldq >= qw and 0 <= q_col
+        if not (n_heads >= 1 and q_out.dtype is src.dtype and q_out.shape == (T, qw) and one == 1 and ldq >= qw and 0 <= q_col
                 and q_col + qw <= k_col <= v_col and device == q_out.get_device()):
             return None
         size, at, own = src.element_size(), q_out.data_ptr(), src.data_ptr()
         apart = at >= own + ((T - 1) * ld + width) * size or at + ((T - 1) * ldq + qw) * size <= own
-        return shape if apart or (at == own + q_col * size and ldq == ld) else None
+        return shape if T == 0 or apart or (at == own + q_col * size and (ldq == ld or T == 1)) else None
     except _NOT_TENSORS:
         return None
 

@@ -85,7 +85,7 @@ def append_both(dtype, H, hkv, dh, ps, requests, turn, dims, mag=1.0, in_place=T
     (6, 3, 48, 8, "pairs", 20), (2, 1, 256, 64, "halves", 256), (3, 3, 15, 16, "pairs", 14), (3, 3, 15, 16, "halves", 6),
     (1, 1, 1, 5, "none", 0), (2, 2, 100, 5, "pairs", 100), (4, 2, 96, 1, "halves", 64), (12, 4, 112, 16, "pairs", 64),
     (3, 1, 176, 48, "none", 0), (25, 25, 64, 16, "none", 0), (4, 2, 128, 64, "pairs", 128), (3, 1, 64, 128, "halves", 64)])
-@pytest.mark.parametrize("requests", [DECODE, PORTIONS], ids=["decode", "portions"])
+@pytest.mark.parametrize("requests", [DECODE, PORTIONS, [(17, 1)]], ids=["decode", "portions", "one row"])
 def test_append(dtype, H, hkv, dh, ps, turn, dims, requests):
     """Numbers and scales are the definition's exactly (both round 64-bit values once); everything outside the rows' pages stays."""
     for in_place in (True, False):
