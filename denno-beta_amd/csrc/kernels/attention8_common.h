@@ -51,12 +51,25 @@ __device__ __forceinline__ void split(const float* v, bf16x8* parts) {
   }
 }
 
-// cap * tanh(s / cap) of a score in units of log2(e): s2 = s log2(e), cap2 = cap log2(e), to_tanh = 2 / cap.  tanh(x) = 1 - 2 / (e^2x + 1),
-// whose error near 0 is some 1e-7 of 1, so the score's is some 1e-7 of cap
-__device__ __forceinline__ float capped(float s2, float cap2, float to_tanh) {
-  const float e = __builtin_amdgcn_exp2f(s2 * to_tanh);
-  return cap2 * fmaf(-2.0f, __builtin_amdgcn_rcpf(e + 1.0f), 1.0f);
-}
+// cap * tanh(s / cap) of a score in units of log2(e): s2 = s log2(e).  With x = s / cap, up to 0.625: tanh(x) = x (1 + x^2 P(x^2)), P of degree four through
+// Chebyshev's nodes in 64 bits, off by 2^-25 of tanh at most; a score that is small beside the cap so comes out as itself, however
+// large the cap.  Elsewhere 1 - 2 / (e^2x + 1), whose error of some 1e-7 is that of tanh itself there (near 0 it would be 1e-7 of the cap,
+// not of the score).  The whole is off by 14 half units of the result's last place at most, hardware's power and reciprocal taken a unit off each.
+struct Cap {      // (made on the host, so that its numbers take no vector registers)
+  float cap2, per_cap, to_tanh;      // cap log2(e) (0: no cap), its inverse, 2 / cap (finite, so that a score of 0 stays 0 under the smallest caps)
+  explicit Cap(float cap) : cap2(cap * LOG2E), per_cap(1.0f / cap2), to_tanh(fminf(2.0f / cap, 3.0e38f)) {}
+  __device__ __forceinline__ float operator()(float s2) const {
+    const float x = s2 * per_cap, z = x * x;
+    float p = -6.104945778808797e-3f;
+    p = fmaf(p, z, 2.100363925867268e-2f);
+    p = fmaf(p, z, -5.3852496893706345e-2f);
+    p = fmaf(p, z, 0.13332782257758075f);
+    p = fmaf(p, z, -0.3333332909943444f);
+    const float e = __builtin_amdgcn_exp2f(s2 * to_tanh);
+    const float far = cap2 * fmaf(-2.0f, __builtin_amdgcn_rcpf(e + 1.0f), 1.0f);
+    return fabsf(x) < 0.625f ? fmaf(s2 * z, p, s2) : far;
+  }
+};
 
 // Results of a row's keys that n_splits workgroups shared out, for every row and head: [rows][heads][n_splits][dh + 2], the running maximum
 // (in units of log2(e)), the sum, the weighted values.  A tile's rows are row0 .. row0 + nrows (no nrows: one).

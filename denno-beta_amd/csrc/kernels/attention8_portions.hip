@@ -29,7 +29,8 @@ struct Args {
   const float* sink_at;
   float* part;      // attend8::Parts' results, with more than one split
   int ldq, ldo, n_pages, max_blocks, n_splits, H, Hkv, page_shift, window, keep, sink;      // pages of 1 << page_shift keys
-  float scale, cap;
+  float scale;
+  Cap cap;
 };
 
 __device__ __forceinline__ u32x4 widen_scaled(uint32_t lo, uint32_t hi, float scale) {
@@ -126,8 +127,8 @@ __global__ __launch_bounds__(64 * RG * KG) __attribute__((amdgpu_waves_per_eu(wa
 #pragma unroll
     for (int i = 0; i < 16; ++i) o[d][i] = 0.f;
   float m_run = LOWEST, l_run = 0.f;
-  const float scale2 = a.scale * LOG2E, cap2 = a.cap * LOG2E, to_tanh = a.cap > 0.f ? 2.0f / a.cap : 0.f;
-  const float per_score = a.cap > 0.f ? 1.0f : scale2;      // what is left to multiply a score with
+  const float scale2 = a.scale * LOG2E;
+  const float per_score = a.cap.cap2 > 0.f ? 1.0f : scale2;      // what is left to multiply a score with
 
   // Steps of 64 KG keys: `kept` ones from the start, then those from the window's first key on.  Step i begins with key_of(i).
   constexpr int STEP = 64 * KG;
@@ -295,11 +296,11 @@ __global__ __launch_bounds__(64 * RG * KG) __attribute__((amdgpu_waves_per_eu(wa
         const int key = kw + 32 * c + 8 * (i / 4) + 4 * g + i % 4;
         return ((there >> (2 * c + i / 8) & 1) != 0) & (key <= my_pos) & ((key >= my_lo) | (key < a.keep));
       };
-      if (a.cap > 0.f) {
+      if (a.cap.cap2 > 0.f) {
 #pragma unroll
         for (int c = 0; c < 2; ++c)
 #pragma unroll
-          for (int i = 0; i < 16; ++i) s[c][i] = capped(s[c][i] * scale2, cap2, to_tanh);
+          for (int i = 0; i < 16; ++i) s[c][i] = a.cap(s[c][i] * scale2);
       }
       if (edge) {
 #pragma unroll
@@ -504,7 +505,7 @@ extern "C" int dn_attention8_portions(const void* q, int ldq, void* out, int ldo
   if (n_tiles == 0) return 0;
   const portions8::Args a = {q, out, static_cast<const uint8_t*>(k_pool), static_cast<const uint8_t*>(v_pool), k_scale, v_scale,
                              block_tables, tile_seq, tile_row0, tile_nrows, tile_pos0, sink_at, part, ldq, ldo, n_pages, max_blocks, n_splits, H, Hkv,
-                             __builtin_ctz(page_size), window, keep, sink, scale, cap};
+                             __builtin_ctz(page_size), window, keep, sink, scale, attend8::Cap(cap)};
   const int rc = dtype == DN_BF16 ? portions8::by_dim<1>(a, n_tiles, dh, rows, groups, stream)
                                   : portions8::by_dim<3>(a, n_tiles, dh, rows, groups, stream);
   if (rc != 0) return rc;

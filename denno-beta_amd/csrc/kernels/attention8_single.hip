@@ -28,7 +28,8 @@ struct Args {
   const float* sink_at;
   float* part;      // attend8::Parts' results
   int ldq, ldo, n_pages, max_blocks, n_splits, H, Hkv, page_shift, window, keep, sink;      // pages of 1 << page_shift keys
-  float scale, cap;
+  float scale;
+  Cap cap;
 };
 
 // a value from the lane 16 away, and the one 32 away
@@ -77,7 +78,7 @@ __global__ __launch_bounds__(WAVES * 64) void kernel(const Args a) {
 #pragma unroll
   for (int d = 0; d < DH16; ++d) o[d] = floatx4{0.f, 0.f, 0.f, 0.f};
   float m_run = LOWEST, l_run = 0.f;
-  const float scale2 = a.scale * LOG2E, cap2 = a.cap * LOG2E, to_tanh = a.cap > 0.f ? 2.0f / a.cap : 0.f;
+  const float scale2 = a.scale * LOG2E;
 
   // the page of the block that begins with `key` and the key's place in it; -1 where the row reads none of it
   auto page_of = [&](int key) {
@@ -123,11 +124,11 @@ __global__ __launch_bounds__(WAVES * 64) void kernel(const Args a) {
 #pragma unroll
       for (int j = 0; j < 4; ++j) s[t][j] *= ks;
     // (every product is read before the first branch behind it: the compiler left out the wait for one that is read behind a branch)
-    if (a.cap > 0.f) {
+    if (a.cap.cap2 > 0.f) {
 #pragma unroll
       for (int t = 0; t < 4; ++t)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) s[t][j] = capped(s[t][j], cap2, to_tanh);
+        for (int j = 0; j < 4; ++j) s[t][j] = a.cap(s[t][j]);
     }
     // a tile at an edge, or with a page that is given back: what the row does not read is -inf, and its values are zeros, whatever
     // stands there (a weight of zero times NaN would be NaN), and so is the scale of a block of which it reads nothing.  The same for
@@ -268,7 +269,7 @@ extern "C" int dn_attention8_single(const void* q, int ldq, void* out, int ldo, 
   if (n_tiles == 0) return 0;
   const single8::Args a = {q, out, static_cast<const uint8_t*>(k_pool), static_cast<const uint8_t*>(v_pool), k_scale, v_scale,
                            block_tables, tile_seq, tile_row0, tile_pos0, sink_at, part, ldq, ldo, n_pages, max_blocks, n_splits, H, Hkv,
-                           __builtin_ctz(page_size), window, keep, sink, scale, cap};
+                           __builtin_ctz(page_size), window, keep, sink, scale, attend8::Cap(cap)};
   const int rc = dtype == DN_BF16 ? single8::by_dim<1>(a, n_tiles, dh, stream) : single8::by_dim<3>(a, n_tiles, dh, stream);
   if (rc != 0) return rc;
   if (n_splits > 1)
