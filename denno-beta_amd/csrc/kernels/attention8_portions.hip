@@ -193,18 +193,20 @@ __global__ __launch_bounds__(64 * RG * KG) __attribute__((amdgpu_waves_per_eu(wa
       for (int w = 0; w < 4; ++w) nan |= (raw.v[u][w] & 0x7f7f7f7fu) + 0x01010101u;
     nan &= 0x80808080u;
     // So would a value beyond the largest number (256 2^120, which a value above 0.97 of it is rounded to): of a page with a scale so large
-    // numbers go in as at most 240, within the rounding that they have had.  What has no page has no scale either.
-    const float v_by = raw.there ? raw.v_by : 1.0f;
-    if (__builtin_amdgcn_ballot_w64(nan != 0 || v_by > LARGEST) != 0) {
+    // numbers go in as at most 240, within the rounding that they have had.  What has no page has no scale either.  A page whose scale is no
+    // finite number (none that was written into a cache is) goes in as one of values that are NaN.
+    const bool scaled = fabsf(raw.v_by) < INFINITY;
+    const float v_by = raw.there && scaled ? raw.v_by : 1.0f;
+    if (__builtin_amdgcn_ballot_w64(nan != 0 || v_by > LARGEST || (raw.there && !scaled)) != 0) {
 #pragma unroll
       for (int u = 0; u < U; ++u)
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
-          raw.v[u][w] &= ~((nan_in(raw.v[u][w]) >> 7) * 0xffu);
+          raw.v[u][w] &= scaled ? ~((nan_in(raw.v[u][w]) >> 7) * 0xffu) : 0u;
           const uint32_t high = v_by > LARGEST ? (((raw.v[u][w] & 0x7f7f7f7fu) + 0x08080808u) & 0x80808080u) >> 7 : 0u;      // from 256 on
           raw.v[u][w] = (raw.v[u][w] & ~(high * 0x7fu)) | high * 0x77u;
         }
-      if (nan != 0 && raw.there) *seen = 1;
+      if (raw.there && (nan != 0 || !scaled)) *seen = 1;
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
@@ -437,8 +439,9 @@ __global__ __launch_bounds__(64 * RG * KG) __attribute__((amdgpu_waves_per_eu(wa
         const int dim = x / 4, first = kt + 16 * (x % 4), page = page_of(kt, 16 * (x % 4), page_entry(kt, 16 * (x % 4)));
         if (page < 0) continue;
         const uint8_t* v = a.v_pool + static_cast<size_t>(page) * page_bytes + (((hk * DH + dim) << a.page_shift) + (first & in_page));
+        const bool scaled = fabsf(a.v_scale[static_cast<size_t>(page) * a.Hkv + hk]) < INFINITY;
         for (int j = 0; j < 16; ++j) {
-          if ((v[j] & 0x7f) != 0x7f) continue;
+          if (scaled && (v[j] & 0x7f) != 0x7f) continue;
           const int key = first + j;
           for (int r = wrow0; r < min(wrow0 + 32, nrows); ++r) {
             const int pos = pos0 + r;

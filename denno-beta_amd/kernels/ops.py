@@ -1082,8 +1082,9 @@ def attention8(q, out, k_pool, v_pool, k_scale, v_scale, block_tables, tiles, n_
     window > 0: the row at position p reads the keys from p - window + 1 on, and with keep_first the request's first so many as well;
     sink: True: one more summand exp(0) under the softmax, or 32-bit [H]: exp(sink[h]), which nothing scales; softcap > 0: a scaled score s
     becomes softcap * tanh(s / softcap).
-    Rows of padding tiles are left as they were.  What stands in places that a row does not read does not reach it, NaN included;
-    a page that is given back (a negative entry) is not read; a row that reads nothing becomes zeros."""
+    Rows of padding tiles are left as they were.  What stands in places that a row does not read does not reach it, NaN included, nor does the
+    scale of a page of which it reads nothing; a page that is given back (a negative entry) is not read; a row that reads nothing becomes
+    zeros.  (A scale that is no finite number, which kv_append8 never writes, leaves the rows that read its page without finite results in its heads.)"""
     shape = _attention8_holds(q, out, k_pool, v_pool, k_scale, v_scale, block_tables, tiles, n_heads)
     if shape is None:
         shape = _pools8(k_pool, v_pool, k_scale, v_scale, "attention8")
