@@ -79,6 +79,11 @@ class CacheStorage:
         return _TORCH[cs.dtype] if cs.dtype is not None else self.kv_dtype
 
     @property
+    def in_8_bits(self):
+        """Whether a group of pages holds 8 bits, with scales."""
+        return any(s is not None for s in self.k_scale)
+
+    @property
     def n_groups(self):
         return len(self.group_specs)
 

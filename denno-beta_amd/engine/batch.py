@@ -36,6 +36,7 @@ class GroupStep:
     tiles_wide: Optional[torch.Tensor] = None   # the same rows in tiles of up to 128
     single_rows: bool = False              # every request brings one row (a pure decode step)
     max_context: int = 0                   # the longest context after this step
+    chosen_by: Optional[Tuple[int, int, int]] = None   # for ops.attention8: what the step and its captured form share out work by (graphs.chosen_by)
 
 
 @dataclass

@@ -32,6 +32,17 @@ def batch_bucket(n: int, limit: int):
     return n
 
 
+def most_context(spec, cache):
+    """The most keys that a request's block table holds: whole pages up to the model's positions (a model that keeps no pages at all, only
+    states, has the model's positions for its bound)."""
+    return min((-(-spec.max_positions // l.page_size) * l.page_size for l in cache.layouts if l.kind == 0), default=spec.max_positions)
+
+
+def context_bucket(longest, most):
+    """Contexts of single rows in buckets of 256, but no bucket beyond what a block table holds."""
+    return min(-(-longest // DECODE_SPLIT) * DECODE_SPLIT, most)
+
+
 class DecodeGraph:
     def __init__(self, runner, batch: int, max_context: int):
         self.manager, self.B, self.max_context = runner.cache.manager, batch, max_context      # (no way back to the runner: no cycle)
@@ -191,8 +202,31 @@ def wanted_rows(entries: Sequence[StepEntry], max_live: int) -> int:
     return wanted if bucket is None else max(wanted, bucket[2])
 
 
+# Attention over the cache in 8 bits shares out its rows and keys to workgroups by a step's rows, tiles and longest context (ops.portions8_plan), and in
+# which order a row's keys are summed depends on that.  So both forms of a step take these from its bucket: the tables' own would differ (a
+# captured step's are padded), and with them the bits; and a captured step that knew no context would not share out keys at all.
+# Contexts in powers of two, rounded down: shares that are too few cost less than shares that are too small.  32 rows of 32 heads of 128
+# behind 30,000 tokens get 8 shares by 16,384 as they would by 30,000.
+def portion_context(longest):
+    return 1 << (longest.bit_length() - 1) if longest >= 128 else 0
+
+
+def portion_chosen_by(T, S, context):
+    """(rows, tiles of up to 128, context): as many tiles as S requests of T rows make on average, each its last one half full."""
+    return (T, max(S, -(-T // 128) + (S - 1) // 2), context)
+
+
+def chosen_by(entries: Sequence[StepEntry], longest: int, max_live: int, most: int):
+    """What a step of these entries shares out its attention by, whether it runs kernel by kernel or captured; None: no graph takes it."""
+    if all(len(e.tokens) == 1 for e in entries):
+        B = batch_bucket(len(entries), max_live)
+        return (B, B, context_bucket(longest, most))
+    bucket = portion_bucket(entries)
+    return None if bucket is None else portion_chosen_by(bucket[0], bucket[1], portion_context(longest))
+
+
 class PortionGraph:
-    def __init__(self, runner, T: int, S: int, R: int):
+    def __init__(self, runner, T: int, S: int, R: int, context: int = 0):
         from .batch import TILE_ROWS, WIDE_TILE_ROWS
         self.manager, self.T, self.S, self.R = runner.cache.manager, T, S, R
         cache, dev = runner.cache, runner.device
@@ -224,7 +258,7 @@ class PortionGraph:
                 groups.append(GroupStep(0, 0, None, None, None))
             else:
                 groups.append(GroupStep(l.page_size, l.window, v(f"sm{g}"), v(f"bt{g}").view(S, self.max_blocks[g]),
-                                        tiles, wide, False, 0))
+                                        tiles, wide, False, 0, portion_chosen_by(T, S, context) if cache.in_8_bits else None))
         self.ctx = StepContext(T=T, S=S, R=R, tokens=v("tokens"), positions=v("positions"),
                                logit_rows=v("logit_rows"), state_slots=v("state_slots"), row_start=v("row_start"),
                                groups=groups, host_row_start=[0] * (S + 1), host_first_pos=[0] * S,
@@ -306,8 +340,9 @@ class DecodeGraphs:
     def __init__(self, runner):
         self._runner = weakref.ref(runner)      # the runner owns these graphs; a reference back would be a cycle
         self.graphs: Dict[Tuple[int, int], DecodeGraph] = {}
-        self.portions: Dict[Tuple[int, int, int], PortionGraph] = {}
-        self.seen: Dict[Tuple[int, int, int], int] = {}      # bucket -> steps that fell into it so far
+        self.portions: Dict[Tuple[int, ...], PortionGraph] = {}
+        self.seen: Dict[Tuple[int, ...], int] = {}      # bucket -> steps that fell into it so far
+        self.contexts: Dict[Tuple[int, int, int], int] = {}      # (T, S, context) -> the least context of the same plans
 
     @property
     def runner(self):
@@ -353,11 +388,7 @@ class DecodeGraphs:
         new_lens = starts + 1
         slots = mgr.reserve_step(rids, new_lens)
         B = batch_bucket(n, runner.options.max_live)
-        # (contexts in buckets of 256, but no bucket beyond what a block table holds: whole pages up to the model's positions)
-        # (a model that keeps no pages at all, only states, has the model's positions for its bound)
-        held = min((-(-spec.max_positions // l.page_size) * l.page_size for l in runner.cache.layouts if l.kind == 0),
-                   default=spec.max_positions)
-        ctx_bucket = min(-(-int(new_lens.max()) // DECODE_SPLIT) * DECODE_SPLIT, held)
+        ctx_bucket = context_bucket(int(new_lens.max()), most_context(spec, runner.cache))
         key = (B, ctx_bucket)
         g = self.graphs.get(key)
         if g is None:
@@ -371,12 +402,37 @@ class DecodeGraphs:
         return out
 
     # -- steps that hold portions ---------------------------------------------------------------------
-    def portion_bucket(self, entries: Sequence[StepEntry]):
-        """(T, S, R) of the bucket that a step with portions falls into, or None if none takes it."""
+    def portion_bucket(self, entries: Sequence[StepEntry], starts=None):
+        """(T, S, R) of the bucket that a step with portions falls into, with a cache in 8 bits (T, S, R, context), or None if none takes it.
+        starts: the requests' lengths before the step, if they are known already."""
         runner = self.runner
         if not runner.model.graph_safe or not runner.options.graph_portions:
             return None
-        return portion_bucket(entries)
+        bucket = portion_bucket(entries)
+        if bucket is None or not runner.cache.in_8_bits:
+            return bucket
+        T, S, _ = bucket
+        if self._same_plans(T, S, portion_context(most_context(runner.spec, runner.cache))) == 0:
+            return bucket + (0,)      # (no context changes anything)
+        if starts is None:
+            starts = runner.cache.manager.lengths(np.asarray([e.rid for e in entries], dtype=np.int64))
+        longest = max([start + len(e.tokens) for e, start in zip(entries, starts.tolist())])
+        return bucket + (self._same_plans(T, S, portion_context(longest)),)
+
+    def _same_plans(self, T, S, context):
+        """The least of the contexts 0, 128, 256, ... up to `context` for which every mixer shares out a step of this bucket as for `context`."""
+        least = self.contexts.get((T, S, context))
+        if least is None:
+            runner = self.runner
+            mixers = [m for b in runner.model.blocks for m in b.mixers() if m.keeps_8_bits]
+
+            def plans(c):
+                return [m.plan_8_bits(*portion_chosen_by(T, S, c), runner.runtime.act_dtype) for m in mixers]
+            least, wanted = context, plans(context)
+            while least > 0 and plans(lower := least // 2 if least > 128 else 0) == wanted:
+                least = lower
+            self.contexts[(T, S, context)] = least
+        return least
 
     def takes_portions(self, entries: Sequence[StepEntry]) -> bool:
         """Whether this step is replayed from a captured graph: its bucket has been met before (and is captured
@@ -394,10 +450,10 @@ class DecodeGraphs:
         a view of the graph's own buffer, which holds them until the same graph is replayed)."""
         runner = self.runner
         mgr = runner.cache.manager
-        key = self.portion_bucket(entries)
         rids = np.asarray([e.rid for e in entries], dtype=np.int64)
         counts = np.asarray([len(e.tokens) for e in entries], dtype=np.int32)
         starts = mgr.lengths(rids)
+        key = self.portion_bucket(entries, starts)
         # (what is wrong with the entries is found before pages are taken: plan_rows raises on them)
         from .batch import plan_rows
         plan_rows(entries, starts.tolist(), runner.spec.vocab, runner.spec.max_positions)

@@ -16,7 +16,7 @@ from ..config import EngineOptions, load_config
 from ..parts import Runtime
 from ..weights import draw_all, load_checkpoint
 from .batch import StepEntry, build_context
-from .graphs import DecodeGraphs, wanted_rows
+from .graphs import DecodeGraphs, chosen_by, most_context, wanted_rows
 
 _ACT = {"bfloat16": torch.bfloat16, "float32": torch.float32}
 _CACHE = {None: None, "float8": torch.float8_e4m3fn}      # None: the activations' dtype
@@ -126,6 +126,11 @@ class ModelRunner:
         if self.device.type == "cuda" and self.model.graph_safe and self.runtime.act_dtype != torch.float32:
             rows = wanted_rows(entries, self.options.max_live)
         ctx = build_context(entries, self.cache, self.spec.vocab, self.spec.max_positions, self.device, rows)
+        if self.device.type == "cuda" and self.model.graph_safe and self.cache.in_8_bits:      # (the captured step's numbers: see chosen_by)
+            longest = max(start + len(e.tokens) for e, start in zip(entries, ctx.host_first_pos))
+            by = chosen_by(entries, longest, self.options.max_live, most_context(self.spec, self.cache))
+            for g in ctx.groups:
+                g.chosen_by = by
         logits = self.model.forward(ctx, self.cache)
         if rows and rows > (wanted := sum([len(e.want) for e in entries])):
             logits = logits[:wanted]

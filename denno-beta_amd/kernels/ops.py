@@ -1041,6 +1041,14 @@ def _portions8_splits(workgroups, groups, dh, max_context, window, keep_first):
     return max(1, min(reach * dh // (64 * groups * 256), (512 if dh <= 64 else 256) // workgroups))
 
 
+def portions8_plan(rows, tiles, max_context, n_heads, dh, dtype, window=0, keep_first=0):
+    """-> (groups of 32 rows, groups of keys of a workgroup, workgroups that a tile's keys are shared out to): how `attention8` shares out a step of `rows`
+    rows in `tiles` tiles of up to 128.  The last two say in which order a row's keys are summed."""
+    of_rows, groups = _portions8_shape(tiles, n_heads, dh, dtype)
+    blocks = min(tiles * 4 // of_rows, tiles + rows // (32 * of_rows))      # (of rows; no more than these have any)
+    return of_rows, groups, _portions8_splits(blocks * n_heads, groups, dh, max_context, window, keep_first)
+
+
 def _attention8_holds(q, out, k_pool, v_pool, k_scale, v_scale, block_tables, tiles, n_heads):
     """The pools' shape if an ordinary call's rows and tables are right, else None."""
     try:
@@ -1070,7 +1078,7 @@ def _attention8_checks(q, out, block_tables, tiles, n_heads, Hkv, dh):
 
 
 def attention8(q, out, k_pool, v_pool, k_scale, v_scale, block_tables, tiles, n_heads, scale, window=0, tiles_wide=None,
-               single_rows=False, max_context=0, sink=False, keep_first=0, softcap=0.0):
+               single_rows=False, max_context=0, sink=False, keep_first=0, softcap=0.0, chosen_by=None):
     """`attention` over a cache in 8 bits as `kv_append8` fills it (that function has the layout of pools and scales): causal attention of
     the batch's rows, with the same tables.
 
@@ -1078,7 +1086,9 @@ def attention8(q, out, k_pool, v_pool, k_scale, v_scale, block_tables, tiles, n_
     h // (H // Hkv).  tiles: int32 [4, n_tiles] = (request, first row, rows <= 16, first position), request < 0: padding;
     tiles_wide: the same rows cut into tiles of up to 128 rows; single_rows: a pure decode step: request s brings row s and is
     tile s, (s or -1, s, 1, position); max_context: the longest context, a must then; with portions it says how far their keys are worth
-    sharing out (0: not at all).
+    sharing out (0: not at all).  chosen_by: (rows, tiles of up to 128 rows, or of one with single_rows, longest context), by which the work is
+    shared out instead of by the tables' own: a row's keys are summed in an order that depends on these, so a step whose tables are padded (a
+    captured one) and the same step without padding have the same bits if they name the same three.
     window > 0: the row at position p reads the keys from p - window + 1 on, and with keep_first the request's first so many as well;
     sink: True: one more summand exp(0) under the softmax, or 32-bit [H]: exp(sink[h]), which nothing scales; softcap > 0: a scaled score s
     becomes softcap * tanh(s / softcap).
@@ -1101,6 +1111,8 @@ def attention8(q, out, k_pool, v_pool, k_scale, v_scale, block_tables, tiles, n_
     T = q.shape[0]
     ldq, ldo = (q.stride(0), out.stride(0)) if T > 1 else (q.shape[1], out.shape[1])
     n_tiles, max_blocks = tiles.shape[1], block_tables.shape[1]
+    if chosen_by is not None and not (len(chosen_by) == 3 and chosen_by[0] >= 1 and chosen_by[1] >= 1 and chosen_by[2] >= 0):
+        raise KernelError(f"attention8: chosen_by {chosen_by}")
     if T == 0 or n_tiles == 0:
         return out
     base = tiles.data_ptr()
@@ -1110,7 +1122,8 @@ def attention8(q, out, k_pool, v_pool, k_scale, v_scale, block_tables, tiles, n_
         _need(n_tiles == T, "attention8: a step of single rows has a tile for every row")
         _need(max_context <= max_blocks * ps, "attention8: max_context exceeds the block tables")
         if aligned:
-            n_splits = _single8_splits(n_tiles, n_heads, Hkv, dh, max_context, window, keep_first)
+            _, tiles_by, context_by = chosen_by or (T, n_tiles, max_context)
+            n_splits = _single8_splits(tiles_by, n_heads, Hkv, dh, context_by, window, keep_first)
             part = torch.empty(n_tiles * n_heads * n_splits * (dh + 2), dtype=torch.float32, device=q.device) if n_splits > 1 else None
             _ok(_lib("cache8").dn_attention8_single(
                 q.data_ptr(), ldq, out.data_ptr(), ldo, k_pool.data_ptr(), v_pool.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
@@ -1124,10 +1137,10 @@ def attention8(q, out, k_pool, v_pool, k_scale, v_scale, block_tables, tiles, n_
         _one_device("attention8", tiles_wide)
         _need(tiles_wide.is_contiguous() and tiles_wide.shape[0] == 4, "attention8: tiles_wide")
         n_wide = tiles_wide.shape[1]
-        rows, groups = _portions8_shape(n_wide, n_heads, dh, q.dtype)
-        # (rows of no tile would have room for results as well)
-        blocks = min(n_wide * 4 // rows, n_wide + T // (32 * rows))      # (of rows; no more than these have any)
-        n_splits = _portions8_splits(blocks * n_heads, groups, dh, max_context, window, keep_first) if 0 < T <= 128 * n_wide else 1
+        rows_by, tiles_by, context_by = chosen_by or (T, n_wide, max_context)
+        rows, groups, n_splits = portions8_plan(rows_by, tiles_by, context_by, n_heads, dh, q.dtype, window, keep_first)
+        if T > 128 * n_wide:      # (rows of no tile would have room for results as well)
+            n_splits = 1
         part = torch.empty(T * n_heads * n_splits * (dh + 2), dtype=torch.float32, device=q.device) if n_splits > 1 else None
         base = tiles_wide.data_ptr()
         _ok(_lib("cache8").dn_attention8_portions(

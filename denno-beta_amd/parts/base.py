@@ -110,6 +110,11 @@ class Part:
     # has k_scale and v_scale, and it calls ops.kv_append8 and ops.attention8
     keeps_8_bits = False
 
+    def plan_8_bits(self, rows, tiles, context, dtype):
+        """Of a mixer that keeps 8 bits: how its attention shares out a step of `rows` rows of `dtype` in `tiles` tiles of up to 128 behind contexts of
+        up to `context`.  Contexts of equal plans share a captured step (engine/graphs.py)."""
+        return context
+
     def param_specs(self) -> List[ParamSpec]:
         return []
 

@@ -120,6 +120,9 @@ class CausalSelfAttention(Part):
     def keeps_8_bits(self):
         return not (self.split or self.prepared)
 
+    def plan_8_bits(self, rows, tiles, context, dtype):
+        return ops.portions8_plan(rows, tiles, context, self.n_heads, self.head_dim, dtype, self.window, self.keep_first)
+
     def bind(self, tensors, runtime):
         super().bind(tensors, runtime)
         self.qkv.bind(tensors)
@@ -233,10 +236,11 @@ class CausalSelfAttention(Part):
             turn = dict(positions=ctx.positions, freq=position.freq, halves=getattr(position, "halves", False), mag=position.mag, q_out=q,
                         q_col=0, n_heads=self.n_heads) if here else {}
             ops.kv_append8(qkv, self.q_width, self.q_width + self.kv_width, g.slot_map, cache.k, cache.v, cache.k_scale, cache.v_scale, **turn)
+        by = {} if g.chosen_by is None else dict(chosen_by=g.chosen_by)
         return ops.attention8(q, torch.empty((h.shape[0], self.q_width), dtype=act, device=h.device), cache.k, cache.v, cache.k_scale,
                               cache.v_scale, g.block_tables, g.tiles, self.n_heads, self.scale, self.window, tiles_wide=g.tiles_wide,
                               single_rows=g.single_rows, max_context=g.max_context, sink=self.sink, keep_first=self.keep_first,
-                              softcap=self.softcap)
+                              softcap=self.softcap, **by)
 
     def forward(self, h, ctx, cache, accumulate_into, stats=None, deferred=None):
         act = self.runtime.act_dtype
