@@ -9,6 +9,15 @@ from ..kernels import ops
 from ..weights.spec import ParamSpec
 from .base import MIXERS, POSITIONS, FixedState, PagedKV, Part
 from .linear import Linear
+from .positions import RotaryHalves, RotaryPairs
+
+
+def turned_in_pages(position, head_dim):
+    """Whether `ops.kv_append8` turns heads of head_dim as position.rotate does: an encoding of the two kinds, with their rotate and turn, whose table
+    is what it turns by.  (One of a user's own goes through its rotate.)"""
+    of = type(position)
+    return (isinstance(position, (RotaryPairs, RotaryHalves)) and of.rotate in (RotaryPairs.rotate, RotaryHalves.rotate)
+            and of.turn in (RotaryPairs.turn, RotaryHalves.turn) and position.head_dim == head_dim and 2 * position.freq.numel() == position.dims > 0)
 
 
 @MIXERS.register("causal_attention")
@@ -223,13 +232,13 @@ class CausalSelfAttention(Part):
         self.out(o, residual=accumulate_into)
 
     def _attend_8_bits(self, h, ctx, cache, g, position):
-        """The projection's rows, keys and values from there to pages in 8 bits (queries and keys turned on the way, where the
-        position encoding has a table of frequencies for whole heads), and the attention over those."""
+        """The projection's rows, keys and values from there to pages in 8 bits (queries and keys turned on the way, where that
+        is what the position encoding does: turned_in_pages), and the attention over those."""
         act = self.runtime.act_dtype
         qkv = self.qkv(h, out_dtype=act)
         q, kv = qkv[:, :self.q_width], qkv[:, self.q_width:self.q_width + self.kv_width]
         turns = position is not None and getattr(position, "rotates", False)
-        here = turns and cache.writes and hasattr(position, "freq") and getattr(position, "head_dim", 0) == self.head_dim and position.dims > 0
+        here = turns and cache.writes and turned_in_pages(position, self.head_dim)
         if turns and not here:
             position.rotate(q, kv, ctx)
         if cache.writes:
