@@ -195,15 +195,16 @@ __global__ __launch_bounds__(64 * RG * KG) __attribute__((amdgpu_waves_per_eu(wa
     // So would a value beyond the largest number (256 2^120, which a value above 0.97 of it is rounded to): of a page with a scale so large
     // numbers go in as at most 240, within the rounding that they have had.  What has no page has no scale either.  A page whose scale is no
     // finite number (none that was written into a cache is) goes in as one of values that are NaN.
-    const bool scaled = fabsf(raw.v_by) < INFINITY;
-    const float v_by = raw.there && scaled ? raw.v_by : 1.0f;
-    if (__builtin_amdgcn_ballot_w64(nan != 0 || v_by > LARGEST || (raw.there && !scaled)) != 0) {
+    float v_by = raw.there ? raw.v_by : 1.0f;
+    if (__builtin_amdgcn_ballot_w64(nan != 0 || !(fabsf(v_by) <= LARGEST)) != 0) {
+      const bool scaled = fabsf(v_by) < INFINITY;
+      v_by = scaled ? v_by : 1.0f;
 #pragma unroll
       for (int u = 0; u < U; ++u)
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
           raw.v[u][w] &= scaled ? ~((nan_in(raw.v[u][w]) >> 7) * 0xffu) : 0u;
-          const uint32_t high = v_by > LARGEST ? (((raw.v[u][w] & 0x7f7f7f7fu) + 0x08080808u) & 0x80808080u) >> 7 : 0u;      // from 256 on
+          const uint32_t high = fabsf(v_by) > LARGEST ? (((raw.v[u][w] & 0x7f7f7f7fu) + 0x08080808u) & 0x80808080u) >> 7 : 0u;      // from 256 on
           raw.v[u][w] = (raw.v[u][w] & ~(high * 0x7fu)) | high * 0x77u;
         }
       if (raw.there && (nan != 0 || !scaled)) *seen = 1;
