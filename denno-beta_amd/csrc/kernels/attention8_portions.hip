@@ -56,7 +56,8 @@ constexpr int waves_per_simd() {      // (with room for one wave only, the compi
   return DH16 * (4 * PARTS + 8) > 128 ? 1 : 2;
 }
 
-template <int DH16, int PARTS, int RG, int KG>
+// CAPPED: scores have a soft cap (a kernel of its own: what the cap takes of registers cost heads of 96, 160 and 256 without one 6 % of their time)
+template <int DH16, int PARTS, int RG, int KG, bool CAPPED>
 __global__ __launch_bounds__(64 * RG * KG) __attribute__((amdgpu_waves_per_eu(waves_per_simd<DH16, PARTS, RG, KG>()))) void kernel(const Args a) {
   constexpr int DH = DH16 * 16, DB = (DH + 31) / 32;
   // elements of a key's row, of a dim's row of 64 keys, 16 bytes of padding each; and 64 bytes more behind every 16 keys, so that the four
@@ -128,7 +129,7 @@ __global__ __launch_bounds__(64 * RG * KG) __attribute__((amdgpu_waves_per_eu(wa
     for (int i = 0; i < 16; ++i) o[d][i] = 0.f;
   float m_run = LOWEST, l_run = 0.f;
   const float scale2 = a.scale * LOG2E;
-  const float per_score = a.cap.cap2 > 0.f ? 1.0f : scale2;      // what is left to multiply a score with
+  const float per_score = CAPPED ? 1.0f : scale2;      // what is left to multiply a score with
 
   // Steps of 64 KG keys: `kept` ones from the start, then those from the window's first key on.  Step i begins with key_of(i).
   constexpr int STEP = 64 * KG;
@@ -299,11 +300,9 @@ __global__ __launch_bounds__(64 * RG * KG) __attribute__((amdgpu_waves_per_eu(wa
         const int key = kw + 32 * c + 8 * (i / 4) + 4 * g + i % 4;
         return ((there >> (2 * c + i / 8) & 1) != 0) & (key <= my_pos) & ((key >= my_lo) | (key < a.keep));
       };
-      if (a.cap.cap2 > 0.f) {
+      if constexpr (CAPPED) {
 #pragma unroll
-        for (int c = 0; c < 2; ++c)
-#pragma unroll
-          for (int i = 0; i < 16; ++i) s[c][i] = a.cap(s[c][i] * scale2);
+        for (int c = 0; c < 2; ++c) a.cap.of<16>(scale2, [&](int i) { return s[c][i]; }, [&](int i, float v) { s[c][i] = v; });
       }
       if (edge) {
 #pragma unroll
@@ -458,19 +457,24 @@ __global__ __launch_bounds__(64 * RG * KG) __attribute__((amdgpu_waves_per_eu(wa
   }
 }
 
-template <int DH16, int PARTS, int RG, int KG>
-static int launch(const Args& a, int n_tiles, hipStream_t stream) {
+template <int DH16, int PARTS, int RG, int KG, bool CAPPED>
+static int launch_as(const Args& a, int n_tiles, hipStream_t stream) {
   constexpr int DH = DH16 * 16, DB = (DH + 31) / 32;
   constexpr int TILES = 2 * KG * (64 * (DH + 8) + 128 + DH * 72) * 2, JOIN = (KG - 1) * 64 * RG * (2 + 16 * DB) * 4;
   constexpr int BYTES = (TILES > JOIN ? TILES : JOIN) + 2 * KG * 4 * 4 + 16;
   static_assert(BYTES <= 160 * 1024, "LDS");
-  auto* fn = &kernel<DH16, PARTS, RG, KG>;
+  auto* fn = &kernel<DH16, PARTS, RG, KG, CAPPED>;
   if (BYTES > 64 * 1024) {
     const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(fn), hipFuncAttributeMaxDynamicSharedMemorySize, BYTES);
     if (e != hipSuccess) return static_cast<int>(e);
   }
   fn<<<dim3(a.H, n_tiles * (4 / RG), a.n_splits), 64 * RG * KG, BYTES, stream>>>(a);
   return 0;
+}
+
+template <int DH16, int PARTS, int RG, int KG>
+static int launch(const Args& a, int n_tiles, hipStream_t stream) {
+  return a.cap.cap2 > 0.f ? launch_as<DH16, PARTS, RG, KG, true>(a, n_tiles, stream) : launch_as<DH16, PARTS, RG, KG, false>(a, n_tiles, stream);
 }
 
 template <int DH16, int PARTS>

@@ -124,12 +124,7 @@ __global__ __launch_bounds__(WAVES * 64) void kernel(const Args a) {
 #pragma unroll
       for (int j = 0; j < 4; ++j) s[t][j] *= ks;
     // (every product is read before the first branch behind it: the compiler left out the wait for one that is read behind a branch)
-    if (a.cap.cap2 > 0.f) {
-#pragma unroll
-      for (int t = 0; t < 4; ++t)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) s[t][j] = a.cap(s[t][j]);
-    }
+    if (a.cap.cap2 > 0.f) a.cap.of<16>(1.0f, [&](int i) { return s[i / 4][i % 4]; }, [&](int i, float v) { s[i / 4][i % 4] = v; });
     // a tile at an edge, or with a page that is given back: what the row does not read is -inf, and its values are zeros, whatever
     // stands there (a weight of zero times NaN would be NaN), and so is the scale of a block of which it reads nothing.  The same for
     // the whole wave.

@@ -31,3 +31,21 @@ def test_caps(dtype, H, hkv, dh, ps, cap):
     for lens, new, how in (([140, 33, 90], [1, 33, 40], {}), ([140, 1, 64], [1] * 3, dict(single_rows=True, max_context=140))):
         case = attention_case(lens, new, H, hkv, dh, ps, dtype, seed=21, q_scale=2.0)
         check(case, H, dh, dtype, cap, (lens, new), **how)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("H,hkv,dh", [(4, 4, 64), (8, 2, 128), (3, 1, 160)])
+def test_a_rows_bits_do_not_depend_on_the_rows_beside_it(dtype, H, hkv, dh):
+    """Tiles of scores that are all small beside the cap go another way than those with larger ones among them: the same bits."""
+    for lens, new, how in (([140], [140], {}), ([140, 90, 33], [1] * 3, dict(single_rows=True, max_context=140))):
+        q, pools, bt, tiles, wide = attention_case(lens, new, H, hkv, dh, 16, dtype, seed=22, q_scale=0.5)
+        on = [p.to(DEV) for p in pools]
+
+        def run(x):
+            x = x.contiguous().to(DEV)
+            return ops().attention8(x, torch.empty_like(x), *on, bt.to(DEV), tiles.to(DEV), H, dh ** -0.5, tiles_wide=wide.to(DEV), softcap=10.0, **how)
+        loud = q.clone()
+        loud[::2] *= 40
+        loud[1:, :dh] *= 40 if how else 1      # (single rows: a wave has a row's heads)
+        a, b = run(q)[1::2], run(loud)[1::2]
+        assert torch.equal(a[:, dh:], b[:, dh:])
