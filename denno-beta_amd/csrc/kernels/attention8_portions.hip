@@ -8,12 +8,15 @@
 //   S^T = K Q^T by v_mfma_f32_32x32x16_bf16: lane (column: a row of q; half g) gets 16 keys of every 32, so the running softmax is
 //   inside a lane but for one exchange between the halves, and its weights are, eight by eight, B operands of
 //   O^T += V^T P^T, whose k-th slots are the keys 16 a + 4 g + {0..3, 8..11}: the values lie in LDS in that order, 16 bytes a read.
-// 32-bit rows: three bfloat16 parts of the queries and of the weights (attend8::split), three products for one.
+// 32-bit rows: three bfloat16 parts of the queries and of the weights (attend8::split), three products for one.  bfloat16 rows: one part of the
+// weights, that is, a weight (at most 1, the largest so exact) rounded to 8 digits in front of the second product, whose operands have no more; the sum under the
+// softmax is of the 32-bit weights.  Beside the rounding of the result itself (0.0016 of its size) it is hardly seen: 0.0017 off 64 bits.
 //
-// Measured: 2,012 rows of 32 heads of 128 behind 2,001 to 8,192 tokens 268 us, 790 TFLOP/s, a third of what the matrix units could do and two thirds of
-// what a large product reaches; they are busy a third of the time, the vector units 40 %, LDS a third, and what keeps the sum of the three from becoming the
-// largest is a wave's own chain from product to softmax to product, with two waves per SIMD.  Two prompts of 1,024 rows of 25 heads of 64 23.5 us, a 32-bit
-// prompt of 1,001 23.0.  Sums of weights by the matrix units, as a product with ones, were slower (16 more registers: 408 -> 658 us undivided).
+// Measured: 1,986 rows of 32 heads of 128 behind 2,001 to 8,192 tokens 262 us, 822 TFLOP/s, a third of what the matrix units could do and two thirds of
+// what a large product reaches.  They are busy a third of the time (33 %), the vector units 46 %, LDS 39 % (a third of that for banks asked for twice), and what keeps
+// the sum of the three from becoming the largest is a wave's own chain from product to softmax to product, with two waves per SIMD, which is what 228
+// registers of 512 leave room for.  Two prompts of 1,024 rows of 25 heads of 64 23.1 us (matrix units 9 %, vector 29 %, LDS 15 %), a 32-bit prompt of 1,001 22.8.
+// Sums of weights by the matrix units, as a product with ones, were slower (16 more registers: 408 -> 658 us undivided).
 #include "attention8_common.h"
 
 namespace portions8 {
@@ -242,8 +245,9 @@ __global__ __launch_bounds__(64 * RG * KG) __attribute__((amdgpu_waves_per_eu(wa
   for (int i = i0; i < i1; ++i, buf ^= 1) {
     // The next tile on its way to LDS, the one after it to registers: the first key group does this in front of its products, the others behind
     // theirs, and products go in front of what the other waves of a SIMD do beside them, so that one wave's products run beside another's
-    // other work: 2,012 rows of 32 heads of 128 behind 2,001 to 8,192 tokens 294 -> 275 us, two prompts of 1,024 25.2 -> 24.3 (groups alone 300 and
-    // 24.8, priorities alone 292 and 24.9; with one key group priorities cost, 271 -> 277).
+    // other work: 2,048 rows of 32 heads of 128 behind 4,000 tokens 204.4 -> 196.1 us (groups alone 214.9, priorities alone 205.5), 1,280 rows 33.0 -> 31.8,
+    // 512 15.0 -> 13.7, two prompts of 1,024 of 25 heads of 64 25.1 -> 24.9.  With one key group there is nobody beside a wave to
+    // take turns with, and priorities cost 2 %.
     auto next = [&]() {
       if (i + 1 < i1) stash(raw, buf ^ 1);
       if (i + 2 < i1) fetch(i + 2, entry, raw);

@@ -10,10 +10,12 @@
 //   O^T = V^T P^T: lane (dim r, group g) reads its dim's 16 values of block g, 16 bytes side by side.
 // No LDS, no exchange between lanes but the maximum's over the four groups, and no number is touched on the way but by the conversion
 // (v_cvt_scalef32_pk_bf16_fp8, two numbers each).  Dims go the same way: 16 bytes of a key are dims 16 g .. 16 g + 15 of a run of 64.
-// 32-bit rows: three bfloat16 parts of the query and of the weights (attend8::split), three products for one.
+// 32-bit rows: three bfloat16 parts of the query and of the weights (attend8::split), three products for one.  bfloat16 rows: one part, the weight
+// rounded to 8 digits, as the second product takes it (the sum under the softmax is of the 32-bit weights): 0.0016 to 0.0018 off 64 bits, of
+// which the result's own rounding is 0.0016.
 //
-// Measured: 64 rows over 500 to 900 keys, 25 heads of 64, 24.7 us, 4.7 TB/s; one row over 131,072 keys, 32 heads over 8 of 128, 47 us, 5.7 TB/s where the
-// memory-side cache has a part of it, 4.9 where it has none; 518 keys of 25 heads 4.9 us, of which 3 are the launch and a trip to memory for the tables.
+// Measured: 64 rows behind 100 to 1,020 tokens, 25 heads of 64, 24.2 us, 4.7 TB/s; one row over 131,072 keys, 32 heads over 8 of 128, 46 us, 5.8 TB/s where the
+// memory-side cache has a part of it, 4.9 where it has none; 518 keys of 25 heads 5.1 us, of which 3 are the launch and a trip to memory for the tables.
 #include "attention8_common.h"
 
 namespace single8 {

@@ -225,7 +225,7 @@ __global__ __launch_bounds__(64 * ANY_TASKS) void any_size_kernel(const Args a) 
 
 // The sizes of models: heads of a multiple of 8, turned entries likewise, pages of a multiple of 16, rows 16-byte aligned.  What bounds
 // these calls is bytes (portions) or a chain of a few trips to memory (single rows), so numbers move eight at a time, and the
-// angles' sines, some 60 instructions of 64 bits each, are made once per workgroup for the eight heads that it turns.
+// angles' sines, some 60 instructions of 64 bits each, are made once per workgroup for the HEADS heads that it turns at a time.
 //   keys and queries: a lane takes a unit of 8 entries of a row: two runs of four, side by side, or with halves half a turn apart;
 //   values: a lane takes two dims and a block of 16 places, so that a dim's 16 numbers, which lie side by side in the page, leave
 //   in one store; what the page holds in that block already is read beside the rows.
@@ -368,7 +368,7 @@ __device__ __forceinline__ void turn_queries(const Args& a, double* turn, int t0
   }
 }
 
-// The rows t0 .. t0 + n, which stand in one page, of eight key heads (group < ceil(Hkv / 8)) or value heads (the groups behind).
+// The rows t0 .. t0 + n, which stand in one page, of HEADS key heads (group < ceil(Hkv / HEADS)) or value heads (the groups behind).
 template <typename T, Turn TURN>
 __device__ __forceinline__ void run_of_rows(const Args& a, double* turn, int* row_in, int group, int t0, int n, int page, int place0, bool odd, int wave,
                                             int lane) {

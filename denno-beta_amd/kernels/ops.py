@@ -1019,12 +1019,14 @@ def _single8_splits(n_tiles, n_heads, Hkv, dh, max_context, window, keep_first):
 
 
 def _portions8_shape(n_tiles, n_heads, dh, dtype):
-    """-> (groups of 32 rows, groups of keys) of a workgroup of the portions' kernel.  Where tiles of 128 rows alone give the chip few
-    workgroups, halves of them, whose keys two groups share out (a row's time is the keys that its wave walks), as long as the chip holds them
-    all: 512 rows of 32 heads of 128 16.8 us and 19.6, two times 512 26.8 and 20.6; 1,001 rows of 16 heads of 96 21.6 and 25.7, 853 of 32 heads 25.5 and
-    21.7; heads up to 64, of which a CU holds two, 2,048 rows of 25 24.5 and 25.6.  Up to two per CU the keys only: 1,280 rows of 32 heads of 128 32.8 us and 43.2
-    (behind thousands of tokens both are level: 97.9 and 93.4, 172.7 and 169.7).  Beyond that neither: three prompts of 1,024, 25 heads of 64, 30.2 us, with
-    keys shared out 37.5.  What does not fit the registers so (heads beyond 128, 32-bit ones beyond 96) goes undivided."""
+    """-> (groups of 32 rows, groups of keys) of a workgroup of the portions' kernel, (4, 1), (4, 2) or (2, 2).  Where tiles of 128 rows alone give the chip
+    few workgroups, their keys go to two groups of waves (a row's time is the keys that its wave walks), and where there are fewer still, halves of
+    tiles do.  Heads of 128, 32 of them, us in (4, 1), (4, 2), (2, 2): 512 rows 20.2, 17.6, 13.9; 640 24.0, 20.6, 17.7; 1,024 35.1, 27.5,
+    34.3; 2,048 68.5, 57.4, 84.2 (a CU holds one workgroup with two groups of keys); 2,176, the first with more tiles than two rounds of one per CU
+    take, 72.9, 73.4, 99.1 (behind 4,000 tokens 286, 277, 384).  Heads of 64, 25 of them, of which a CU holds two: 1,024 rows 25.6, 19.9, 16.7; 1,536
+    36.2, 26.7, 23.5; 2,048 46.3, 35.0, 35.0; 2,560 56.3, 47.7, 47.2; 3,584 78.3, 86.9, 84.4: from 400 tiles on the two with key groups are within 3 % of each other (two
+    prompts of 1,152 28.7 and 27.4), so that it does not matter where between 400 and 500 one takes over.  What does not fit the registers so (heads
+    beyond 128, 32-bit ones beyond 96) goes undivided."""
     blocks = n_tiles * n_heads
     if dh > (128 if dtype is torch.bfloat16 else 96) or blocks > 512:
         return 4, 1
