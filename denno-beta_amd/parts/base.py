@@ -107,7 +107,7 @@ class Part:
     graph_safe = False
     libraries = ()     # kernel libraries (names in build.LIBRARIES) beyond the ones every model needs
     # a mixer that writes and reads pages in 8 bits where the engine keeps them so (EngineOptions.cache_dtype): its CacheView then
-    # has k_scale and v_scale, and it calls ops.kv_append8 and ops.attention8
+    # has k_scale and v_scale, and it calls ops.kv_append8 and ops.attention8 (with the GroupStep's chosen_by, where there is one)
     keeps_8_bits = False
 
     def plan_8_bits(self, rows, tiles, context, dtype):
